@@ -21,7 +21,9 @@ FLAG_EXACT_SELECT, FLAG_NO_TMA, FLAG_NO_SPLIT = 1, 2, 4
 QUASAR_NOALLOC_WORKSPACE_BYTES = 32 << 20  # include/quasar_sampler.h
 SYNTH_NORMAL, SYNTH_GUMBEL_PEAK, SYNTH_ZIPF = 0, 1, 2
 
-# Every symbol include/quasar_sampler.h declares, with (argtypes, restype).
+F32, F16, BF16 = 0, 1, 2  # include/quasar_losses.h
+
+# Every symbol the headers under include/ declare, with (argtypes, restype).
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _I64 = ctypes.c_int64
@@ -61,6 +63,12 @@ SIGNATURES = {
     "quasar_synth_hist": ([_U64, _I64, _I, _I, _I, _P, _P], _I),
     "quasar_synth_uniform": ([_U64, _I64, _I, _F, _F, _P, _P], _I),
     "quasar_selftest_exp": ([_P, _P, _I, _I, _P], _I),
+    # include/quasar_losses.h
+    "quasar_token_logprobs": ([_P, _I, _I64, _I, _I, _P, _F, _P, _P, _P, _P], _I),
+    "quasar_token_logprobs_grad": ([_P, _I, _I64, _I, _I, _P, _F, _P, _P, _P, _P, _P, _I64, _P], _I),
+    "quasar_policy_loss": ([_P, _I, _I64, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _P], _I),
+    "quasar_preference_loss": ([_P, _I, _I64, _I, _I, _P, _P, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64,
+                                _P], _I),
 }
 
 _lib: ctypes.CDLL | None = None

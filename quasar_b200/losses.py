@@ -1,0 +1,317 @@
+"""Log-probabilities of given tokens and the losses made of them, over rows of logits.
+
+The Python side of include/quasar_losses.h: ``token_logprobs`` and its gradient, the clipped
+policy loss and the paired preference loss, each over a [rows, V] CUDA tensor of logits
+(float32, float16 or bfloat16, unit column stride) and int32 targets, as ``pick_batch`` writes
+them. A target below 0 marks a row that takes no part (outputs 0, a gradient of zeros).
+
+Losses return their gradient into the logits with them, so one call is a forward and a backward
+pass; a model goes on from there with ``logits.backward(result.grad)``. Nothing is registered
+with autograd. Outputs are allocated on the stream of the call, or given (``out=``, ``grad=``)
+and used again. torch is used only for device memory and streams.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import NamedTuple, Optional
+
+from ._lib import BF16, F16, F32, check, lib
+
+_DTYPES = {}  # torch dtype -> the C constant; filled at the first call, torch being imported only then
+
+
+class PolicyParams(ctypes.Structure):
+    """ctypes twin of quasar_policy_params."""
+    _fields_ = [("temperature", ctypes.c_float), ("clip_low", ctypes.c_float), ("clip_high", ctypes.c_float),
+                ("kl_coef", ctypes.c_float), ("entropy_coef", ctypes.c_float), ("grad_scale", ctypes.c_float)]
+
+
+class PreferenceParams(ctypes.Structure):
+    """ctypes twin of quasar_preference_params."""
+    _fields_ = [("temperature", ctypes.c_float), ("beta", ctypes.c_float), ("label_smoothing", ctypes.c_float),
+                ("grad_scale", ctypes.c_float), ("length_normalize", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
+class TokenLogprobs(NamedTuple):
+    logprob: torch.Tensor             # [rows] float32
+    entropy: Optional[torch.Tensor]   # [rows] float32, or None
+    stats: torch.Tensor               # [rows, 2] float32: the row's largest logit, its sum of exp((l - max) / T)
+
+
+class PolicyLoss(NamedTuple):
+    loss: torch.Tensor                # [] float32
+    logprob: torch.Tensor             # [rows] float32
+    entropy: Optional[torch.Tensor]   # [rows] float32, or None
+    row_loss: torch.Tensor            # [rows] float32, without the weights
+    grad: Optional[torch.Tensor]      # [rows, V] of the logits' type, or None
+
+
+class PreferenceLoss(NamedTuple):
+    loss: torch.Tensor                # [] float32
+    pair_loss: torch.Tensor           # [pairs] float32
+    seq_logprob: torch.Tensor         # [2 * pairs] float32: chosen, rejected, chosen, ...
+    logprob: torch.Tensor             # [rows] float32
+    stats: torch.Tensor               # [rows, 2] float32, as TokenLogprobs.stats
+    row_grad: torch.Tensor            # [rows] float32: d loss / d logprob, times grad_scale
+    grad: Optional[torch.Tensor]      # [rows, V] of the logits' type, or None
+
+
+def _rows(logits, targets):
+    """Checks logits and targets; returns (rows, V, the C dtype)."""
+    import torch
+    if not _DTYPES:
+        _DTYPES.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
+    if logits.dim() != 2 or logits.dtype not in _DTYPES:
+        raise ValueError("logits must be a [rows, V] float32, float16 or bfloat16 tensor")
+    if not logits.is_cuda:
+        raise ValueError("logits must be a CUDA tensor")
+    rows, V = logits.shape
+    if logits.stride(1) != 1 and V > 1:
+        raise ValueError("logits must have unit column stride")
+    if rows > 1 and logits.stride(0) < V:
+        raise ValueError("rows of logits must not overlap")
+    _vec(targets, "targets", (rows,), torch.int32, logits)
+    return rows, V, _DTYPES[logits.dtype]
+
+
+def _vec(t, name, shape, dtype, logits):
+    if t.shape != shape or t.dtype != dtype or t.device != logits.device or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {list(shape)} on {logits.device}, got "
+                         f"{t.dtype} {list(t.shape)} on {t.device}")
+
+
+def _ld(t):
+    """Row stride in elements (a tensor of one row or none may have any)."""
+    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
+
+
+def _like(logits):
+    """A gradient buffer of the logits' shape whose rows have the 16-byte phase of the logits' rows."""
+    import torch
+    rows, V = logits.shape
+    ld, size = _ld(logits), logits.element_size()
+    if ld == V and logits.data_ptr() % 16 == 0:
+        return torch.empty((rows, V), dtype=logits.dtype, device=logits.device)
+    per = 16 // size
+    first = logits.data_ptr() % 16 // size
+    ld = V + (ld - V) % per  # the shortest stride with the same phases
+    flat = torch.empty(first + rows * ld, dtype=logits.dtype, device=logits.device)
+    return flat.as_strided((rows, V), (ld, 1), first)
+
+
+def _check_grad(grad, logits):
+    if grad.shape != logits.shape or grad.dtype != logits.dtype or grad.device != logits.device:
+        raise ValueError(f"the gradient must be a {logits.dtype} tensor of shape {list(logits.shape)} on {logits.device}")
+    if (grad.stride(1) != 1 and grad.shape[1] > 1) or (grad.shape[0] > 1 and grad.stride(0) < grad.shape[1]):
+        raise ValueError("the gradient must have unit column stride and rows that do not overlap")
+
+
+def _p(t):
+    return None if t is None else t.data_ptr()
+
+
+class _On:
+    """Makes the logits' device and the stream of the call current, and keeps the call's tensors from being
+    handed out again before that stream is done with them."""
+
+    def __init__(self, logits, stream, tensors):
+        self.device = logits.device.index
+        self.stream = stream
+        self.tensors = tensors
+
+    def __enter__(self):
+        import torch
+        self.before = None
+        if torch.cuda.current_device() != self.device:
+            self.before = torch.cuda.current_device()
+            torch.cuda.set_device(self.device)
+        current = torch.cuda.current_stream(self.device)
+        self.back = None
+        if self.stream is not None and self.stream != current:
+            if self.stream.device.index != self.device:
+                self.__exit__()
+                raise ValueError(f"the stream is on {self.stream.device}, the logits on cuda:{self.device}")
+            for t in self.tensors:
+                if t is not None:
+                    t.record_stream(self.stream)
+            self.back = current
+            torch.cuda.set_stream(self.stream)
+            current = self.stream
+        return current.cuda_stream
+
+    def __exit__(self, *exc):
+        import torch
+        if getattr(self, "back", None) is not None:
+            torch.cuda.set_stream(self.back)
+        if self.before is not None:
+            torch.cuda.set_device(self.before)
+        return False
+
+
+def token_logprobs(logits, targets, *, temperature: float = 1.0, entropy: bool = False,
+                   out: Optional[TokenLogprobs] = None, stream=None) -> TokenLogprobs:
+    """Log-probability of each row's target under softmax(logits / temperature), and on request the row's entropy.
+
+    targets: [rows] int32; below 0: the row is not read and its outputs are 0.
+    out: a TokenLogprobs of an earlier call whose tensors are written again (its entropy as ``entropy`` asks).
+    Launches on ``stream`` (a torch.cuda.Stream; default: the current stream).
+    """
+    import torch
+    rows, V, dt = _rows(logits, targets)
+    if out is not None:
+        _vec(out.logprob, "out.logprob", (rows,), torch.float32, logits)
+        _vec(out.stats, "out.stats", (rows, 2), torch.float32, logits)
+        if entropy != (out.entropy is not None):
+            raise ValueError("out.entropy must be a tensor if entropy is asked for, and None if not")
+        if entropy:
+            _vec(out.entropy, "out.entropy", (rows,), torch.float32, logits)
+    with _On(logits, stream, (logits, targets, *(out or ()))) as st:
+        if out is None:
+            dev = logits.device
+            out = TokenLogprobs(torch.empty(rows, device=dev, dtype=torch.float32),
+                                torch.empty(rows, device=dev, dtype=torch.float32) if entropy else None,
+                                torch.empty((rows, 2), device=dev, dtype=torch.float32))
+        check(lib().quasar_token_logprobs(_p(logits), dt, _ld(logits), rows, V, _p(targets), temperature,
+                                          _p(out.logprob), _p(out.entropy), _p(out.stats), st),
+              "quasar_token_logprobs")
+    return out
+
+
+def token_logprobs_grad(logits, targets, stats, grad_logprob, *, entropy=None, grad_entropy=None,
+                        temperature: float = 1.0, out=None, stream=None):
+    """Gradient into the logits of sum(grad_logprob * logprob + grad_entropy * entropy).
+
+    stats (and entropy, with grad_entropy): what ``token_logprobs`` gave for the same logits, targets and
+    temperature. out: a tensor of the logits' shape and type to write, which may be ``logits`` itself.
+    Returns the gradient, of the logits' type.
+    """
+    import torch
+    rows, V, dt = _rows(logits, targets)
+    _vec(stats, "stats", (rows, 2), torch.float32, logits)
+    _vec(grad_logprob, "grad_logprob", (rows,), torch.float32, logits)
+    if (entropy is None) != (grad_entropy is None):
+        raise ValueError("pass entropy and grad_entropy together")
+    if entropy is not None:
+        _vec(entropy, "entropy", (rows,), torch.float32, logits)
+        _vec(grad_entropy, "grad_entropy", (rows,), torch.float32, logits)
+    if out is not None:
+        _check_grad(out, logits)
+    with _On(logits, stream, (logits, targets, stats, grad_logprob, entropy, grad_entropy, out)) as st:
+        if out is None:
+            out = _like(logits)
+        check(lib().quasar_token_logprobs_grad(_p(logits), dt, _ld(logits), rows, V, _p(targets), temperature,
+                                               _p(stats), _p(entropy), _p(grad_logprob), _p(grad_entropy), _p(out),
+                                               _ld(out), st), "quasar_token_logprobs_grad")
+    return out
+
+
+def _grad_arg(grad, logits):
+    import torch
+    if isinstance(grad, torch.Tensor):
+        _check_grad(grad, logits)
+    elif grad is not True and grad is not False:
+        raise ValueError("grad must be True (allocate), False (none) or a tensor to write")
+
+
+def policy_loss(logits, targets, old_logprob, advantage, *, ref_logprob=None, weight=None, temperature: float = 1.0,
+                clip_low: float = 0.2, clip_high: float = 0.2, kl_coef: float = 0.0, entropy_coef: float = 0.0,
+                grad_scale: float = 1.0, entropy: bool = False, grad=True, out: Optional[PolicyLoss] = None,
+                stream=None) -> PolicyLoss:
+    """Clipped policy loss of the rows' tokens, with an optional KL term and entropy bonus, and its gradient.
+
+    ratio = exp(logprob - old_logprob), u = ref_logprob - logprob:
+      row_loss = -min(ratio * A, clip(ratio, 1 - clip_low, 1 + clip_high) * A) + kl_coef * (exp(u) - u - 1)
+                 - entropy_coef * entropy
+      loss     = sum(weight * row_loss)
+    old_logprob, advantage, ref_logprob, weight: [rows] float32. weight None: 1/rows each; a weight of 0 leaves the
+    row out like a negative target. entropy: return the rows' entropies (they are returned whenever entropy_coef
+    is not 0). grad: True to allocate the gradient, a tensor to write (``logits`` itself: in place), False for
+    none. grad_scale multiplies the gradient, not the loss. out: a PolicyLoss of an earlier call whose tensors
+    other than grad are written again.
+    """
+    import torch
+    rows, V, dt = _rows(logits, targets)
+    f32 = torch.float32
+    _vec(old_logprob, "old_logprob", (rows,), f32, logits)
+    _vec(advantage, "advantage", (rows,), f32, logits)
+    if ref_logprob is not None:
+        _vec(ref_logprob, "ref_logprob", (rows,), f32, logits)
+    elif kl_coef != 0.0:
+        raise ValueError("kl_coef needs ref_logprob")
+    if weight is not None:
+        _vec(weight, "weight", (rows,), f32, logits)
+    want = entropy or entropy_coef != 0.0
+    _grad_arg(grad, logits)
+    if out is not None:
+        _vec(out.loss, "out.loss", (), f32, logits)
+        _vec(out.logprob, "out.logprob", (rows,), f32, logits)
+        _vec(out.row_loss, "out.row_loss", (rows,), f32, logits)
+        if want != (out.entropy is not None):
+            raise ValueError("out.entropy must be a tensor if the entropy is computed, and None if not")
+        if want:
+            _vec(out.entropy, "out.entropy", (rows,), f32, logits)
+    prm = PolicyParams(temperature, clip_low, clip_high, kl_coef, entropy_coef, grad_scale)
+    buf = grad if isinstance(grad, torch.Tensor) else None
+    with _On(logits, stream, (logits, targets, old_logprob, advantage, ref_logprob, weight, buf, *(out or ()))) as st:
+        dev = logits.device
+        if out is None:
+            out = PolicyLoss(torch.empty((), device=dev, dtype=f32), torch.empty(rows, device=dev, dtype=f32),
+                             torch.empty(rows, device=dev, dtype=f32) if want else None,
+                             torch.empty(rows, device=dev, dtype=f32), None)
+        if grad is True:
+            buf = _like(logits)
+        check(lib().quasar_policy_loss(_p(logits), dt, _ld(logits), rows, V, _p(targets), _p(old_logprob),
+                                       _p(advantage), _p(ref_logprob), _p(weight), ctypes.addressof(prm),
+                                       _p(out.logprob), _p(out.entropy), _p(out.row_loss), _p(out.loss), _p(buf),
+                                       0 if buf is None else _ld(buf), st), "quasar_policy_loss")
+    return out._replace(grad=buf)
+
+
+def preference_loss(logits, targets, cu_seqlens, *, ref_logprob=None, pair_weight=None, temperature: float = 1.0,
+                    beta: float = 0.1, label_smoothing: float = 0.0, length_normalize: bool = False,
+                    grad_scale: float = 1.0, grad=True, out: Optional[PreferenceLoss] = None,
+                    stream=None) -> PreferenceLoss:
+    """Preference loss over pairs of packed sequences (chosen, rejected, chosen, ...) and its gradient.
+
+    cu_seqlens: [2 * pairs + 1] int32 row offsets; a row counts if its target is not negative. With a sequence's
+    score the sum (length_normalize: the mean) of its log-probabilities less ref_logprob ([2 * pairs] float32):
+      x         = beta * (score_chosen - score_rejected)
+      pair_loss = -(1 - label_smoothing) * ln sigmoid(x) - label_smoothing * ln sigmoid(-x)
+      loss      = sum(pair_weight * pair_loss)                  (pair_weight None: 1/pairs each)
+    grad, grad_scale, out: as for ``policy_loss``.
+    """
+    import torch
+    rows, V, dt = _rows(logits, targets)
+    f32 = torch.float32
+    if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] % 2 == 0:
+        raise ValueError("cu_seqlens must have 2 * pairs + 1 offsets")
+    n = cu_seqlens.shape[0] - 1
+    _vec(cu_seqlens, "cu_seqlens", (n + 1,), torch.int32, logits)
+    if ref_logprob is not None:
+        _vec(ref_logprob, "ref_logprob", (n,), f32, logits)
+    if pair_weight is not None:
+        _vec(pair_weight, "pair_weight", (n // 2,), f32, logits)
+    _grad_arg(grad, logits)
+    if out is not None:
+        for name, shape in (("loss", ()), ("pair_loss", (n // 2,)), ("seq_logprob", (n,)), ("logprob", (rows,)),
+                            ("stats", (rows, 2)), ("row_grad", (rows,))):
+            _vec(getattr(out, name), "out." + name, shape, f32, logits)
+    prm = PreferenceParams(temperature, beta, label_smoothing, grad_scale, 1 if length_normalize else 0, 0)
+    buf = grad if isinstance(grad, torch.Tensor) else None
+    with _On(logits, stream, (logits, targets, cu_seqlens, ref_logprob, pair_weight, buf, *(out or ()))) as st:
+        dev = logits.device
+        if out is None:
+            e = lambda *shape: torch.empty(shape, device=dev, dtype=f32)  # noqa: E731
+            out = PreferenceLoss(e(), e(n // 2), e(n), e(rows), e(rows, 2), e(rows), None)
+        if grad is True:
+            buf = _like(logits)
+        check(lib().quasar_preference_loss(_p(logits), dt, _ld(logits), rows, V, _p(targets), _p(cu_seqlens), n // 2,
+                                           _p(ref_logprob), _p(pair_weight), ctypes.addressof(prm), _p(out.logprob),
+                                           _p(out.seq_logprob), _p(out.pair_loss), _p(out.loss), _p(out.stats),
+                                           _p(out.row_grad), _p(buf), 0 if buf is None else _ld(buf), st),
+              "quasar_preference_loss")
+    return out._replace(grad=buf)
+
+
+__all__ = ["TokenLogprobs", "PolicyLoss", "PreferenceLoss", "PolicyParams", "PreferenceParams", "token_logprobs",
+           "token_logprobs_grad", "policy_loss", "preference_loss"]
