@@ -102,6 +102,7 @@ int quasar_policy_loss(const void* d_logits, int dtype, int64_t ld, int rows, in
         a.adv = d_advantage;
         a.ref_lp = d_ref_logprob;
         a.weight = d_weight;
+        a.mean = 1.0 / rows;
         a.clip_lo = params->clip_low;
         a.clip_hi = params->clip_high;
         a.kl = params->kl_coef;

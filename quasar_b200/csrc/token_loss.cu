@@ -1,31 +1,38 @@
 // token_loss.cu - kernels of the token log-probabilities and of the losses
 // made of them (include/quasar_losses.h).
 //
-// The mathematics: with M the largest logit of a row and d = l - M, the row's
-// softmax needs S = sum 2^(d*k), k = log2(e)/T, and its entropy also
-// Q = sum 2^(d*k) * d*k:  logprob = ln2 * (d_target*k - log2 S),
-// entropy = ln2 * (log2 S - Q/S). M is not known while the row streams, so a
-// thread sums against a reference that trails its running maximum and moves
-// (one rescale of the sums) only when a logit passes it by 2^LAG: terms stay
-// below 2^LAG, far inside fp32, and rescales are rare. Differences are taken
-// before the multiply by k, so that rows at the type's lowest value (a fully
-// masked row) do not overflow.
+// The mathematics: with k = log2(e) / T, M the largest logit of a row, R = M*k
+// rounded to fp32 and t = l*k - R (one fused multiply-add), the row's softmax
+// needs S = sum 2^t and its entropy also Q = sum 2^t * t:
+//   logprob = ln2 * t_target - ln S,  entropy = ln S - ln2 * Q / S,
+//   p_v = 2^t / S.
+// M is not known while the row streams, so a thread sums against a reference
+// that trails its running maximum and moves (one rescale of the sums) only
+// when a logit passes it by 2^LAG: terms stay below 2^LAG, far inside fp32,
+// and rescales are rare. A row whose M*k overflows (masked throughout by the
+// type's lowest value) is summed over again with t = (l - M) * k.
+//
+// What bounds it: HBM for fp32 (4 bytes an element and pass); for 16-bit
+// types one exponential per element and pass on the special-function unit
+// (16 a clock and SM) takes 0.7 of the time that the bytes take.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <float.h>
 #include <math.h>
 
+#include <mutex>
+
 #include "common.cuh"
+#include "ptx.cuh"
 #include "token_loss.cuh"
 
 namespace qs {
 namespace loss {
 
-constexpr int NT = 256;  // threads per CTA
-constexpr int NW = NT / 32;
-constexpr int U = 4;     // 16-byte loads in flight per thread
-constexpr int MAXC = 8;  // CTAs of a row's cluster at most
-constexpr float LAG = 20.0f;
+constexpr int U = 4;           // 16-byte loads in flight per thread
+constexpr int MAXC = 8;        // CTAs of a row's cluster at most (the portable limit)
+constexpr float LAG = 20.0f;   // powers of two that a term may stand above the reference
+constexpr float WIDE = 1e37f;  // rows whose |M| * k passes this are summed with differences taken first
 constexpr float NEG = -FLT_MAX;
 constexpr double LN2 = 0.6931471805599453094;
 
@@ -110,75 +117,383 @@ __device__ __forceinline__ Span span_of(const T* row, int V) {
     return s;
 }
 
+
+// Part `part` of `parts` of a row's packs, and the edge element (of part 0)
+// that this thread takes: at most 2 * (N - 1) of them, one a thread.
+struct Slice {
+    int head, lo, n;  // packs [lo, lo + n)
+    int edge;         // element, or -1
+};
+template <typename T>
+__device__ __forceinline__ Slice slice_of(const T* row, int V, int part, int parts) {
+    const Span sp = span_of(row, V);
+    const int tid = threadIdx.x;
+    Slice s;
+    s.head = sp.head;
+    s.lo = (int)((unsigned)sp.packs * (unsigned)part / (unsigned)parts);
+    s.n = (int)((unsigned)sp.packs * (unsigned)(part + 1) / (unsigned)parts) - s.lo;
+    s.edge = part == 0 && tid < sp.head + sp.tail ? (tid < sp.head ? tid : V - sp.tail + (tid - sp.head)) : -1;
+    return s;
+}
+
+// Largest element of some packs (NaN is left to the sums).
+template <int P>
+__device__ __forceinline__ float packs_max(const uint4 (&p)[P], float*) {
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < P; i++) {
+        m = max3(m, __uint_as_float(p[i].x), __uint_as_float(p[i].y));
+        m = max3(m, __uint_as_float(p[i].z), __uint_as_float(p[i].w));
+    }
+    return m;
+}
+#define QS_MAX2(op, d, a, b) asm(op " %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b))
+template <int P>
+__device__ __forceinline__ float packs_max(const uint4 (&p)[P], __nv_bfloat16*) {
+    uint32_t m = Type<__nv_bfloat16>::NEG_INF;
+#pragma unroll
+    for (int i = 0; i < P; i++) {
+        uint32_t a, b;
+        QS_MAX2("max.bf16x2", a, p[i].x, p[i].y);
+        QS_MAX2("max.bf16x2", b, p[i].z, p[i].w);
+        QS_MAX2("max.bf16x2", a, a, b);
+        QS_MAX2("max.bf16x2", m, m, a);
+    }
+    return fmaxf(__uint_as_float(m << 16), __uint_as_float(m & 0xFFFF0000u));
+}
+template <int P>
+__device__ __forceinline__ float packs_max(const uint4 (&p)[P], __half*) {
+    uint32_t m = Type<__half>::NEG_INF;
+#pragma unroll
+    for (int i = 0; i < P; i++) {
+        uint32_t a, b;
+        QS_MAX2("max.f16x2", a, p[i].x, p[i].y);
+        QS_MAX2("max.f16x2", b, p[i].z, p[i].w);
+        QS_MAX2("max.f16x2", a, a, b);
+        QS_MAX2("max.f16x2", m, m, a);
+    }
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&m));
+    return fmaxf(f.x, f.y);
+}
+#undef QS_MAX2
+
 // ---- running sums of one thread -------------------------------------------
 
 struct Acc {
-    float ref;  // what the sums are taken against (NEG: nothing yet)
-    float mx;   // largest element
-    float s, q;
+    float c;     // scaled reference that the sums are taken against (NEG: none yet)
+    float mx;    // largest element
+    f32x2 s, q;  // sums of 2^t and of 2^t * t, t = l * k - c, in two lanes
 };
 
-// Adds the N elements of x (their maximum is mx).
-template <bool ENT, int N>
-__device__ __forceinline__ void add(Acc& a, const float (&x)[N], float k) {
-    float mx = x[0];
-#pragma unroll
-    for (int i = 1; i < N; i++) mx = fmaxf(mx, x[i]);
-    if ((mx - a.ref) * k > LAG) {
-        const float d = fmaxf((a.ref - mx) * k, -1e30f);  // finite, for sums still at 0
-        const float f = ex2_approx(d);
-        if (ENT) a.q = (a.q + a.s * d) * f;
-        a.s *= f;
-        a.ref = mx;
-    }
+__device__ __forceinline__ Acc acc_new() { return Acc{NEG, -INFINITY, pack2(0.0f, 0.0f), pack2(0.0f, 0.0f)}; }
+
+// Moves the reference up to the scaled maximum of what comes next.
+template <bool ENT>
+__device__ __forceinline__ void acc_raise(Acc& a, float mx, float k) {
     a.mx = fmaxf(a.mx, mx);
-    const f32x2 nref = pack2(-a.ref, -a.ref), kk = pack2(k, k);
-    f32x2 s = pack2(0.0f, 0.0f), q = pack2(0.0f, 0.0f);
+    if (fmaf(mx, k, -a.c) > LAG) {
+        const float c = mx * k, d = fmaxf(a.c - c, -1e30f);  // finite, for sums still at 0
+        const float f = ex2_approx(d);
+        const f32x2 ff = pack2(f, f);
+        if (ENT) a.q = mul2(fma2(a.s, pack2(d, d), a.q), ff);
+        a.s = mul2(a.s, ff);
+        a.c = c;
+    }
+}
+
+template <bool ENT, int N>
+__device__ __forceinline__ void acc_add(Acc& a, const float (&x)[N], float k) {
+    const f32x2 nc = pack2(-a.c, -a.c), kk = pack2(k, k);
 #pragma unroll
     for (int i = 0; i < N; i += 2) {
+        const f32x2 t = fma2(pack2(x[i], x[i + 1]), kk, nc);
         float t0, t1;
-        unpack2(mul2(add2(pack2(x[i], x[i + 1]), nref), kk), t0, t1);
+        unpack2(t, t0, t1);
         const f32x2 e = pack2(ex2_approx(t0), ex2_approx(t1));
-        s = add2(s, e);
+        a.s = add2(a.s, e);
         // a term of 0 at t = -inf must not become NaN; NaN stays in e
-        if (ENT) q = fma2(e, pack2(fmaxf(t0, -200.0f), fmaxf(t1, -200.0f)), q);
-    }
-    float a0, a1;
-    unpack2(s, a0, a1);
-    a.s += a0 + a1;
-    if (ENT) {
-        unpack2(q, a0, a1);
-        a.q += a0 + a1;
+        if (ENT) a.q = fma2(e, pack2(fmaxf(t0, -200.0f), fmaxf(t1, -200.0f)), a.q);
     }
 }
 
-// (max, sum, Q) of a set of elements, the sums taken against the maximum.
-struct Part {
-    double s, q;
-    float m;
-    float pad;
+template <typename T, bool ENT, int P>
+__device__ __forceinline__ void acc_packs(Acc& a, const uint4 (&p)[P], float k) {
+    acc_raise<ENT>(a, packs_max(p, (T*)nullptr), k);
+#pragma unroll
+    for (int i = 0; i < P; i++) {
+        float x[Type<T>::N];
+        widen(p[i], x, (T*)nullptr);
+        acc_add<ENT>(a, x, k);
+    }
+}
+
+template <bool ENT>
+__device__ __forceinline__ void acc_one(Acc& a, float x, float k) {
+    const float y[2] = {x, -INFINITY};
+    acc_raise<ENT>(a, x, k);
+    acc_add<ENT>(a, y, k);
+}
+
+// (max, sum, Q) of a set of elements, the sums against the scaled maximum.
+struct __align__(16) Part {
+    float m, s, q, pad;
 };
 
-// Brings sums taken against `from` to `to` (>= from where the sums are not 0).
-template <typename F>
-__device__ __forceinline__ void rebase(F& s, F& q, float from, float to, float k) {
-    const float base = to == -INFINITY ? 0.0f : to;
-    const float d = fmaxf((from - base) * k, -1e30f);
-    const float f = from == to ? 1.0f : ex2_approx(d);
-    q = (q + s * (F)(from == to ? 0.0f : d)) * (F)f;
-    s *= (F)f;
+// The reference of sums with maximum m (finite for a maximum of the lowest
+// value or -inf, whose sums are 0).
+__device__ __forceinline__ float scaled(float m, float k) { return fmaxf(m * k, NEG); }
+
+// Brings sums taken against the scaled reference `from` to the one of `m`.
+__device__ __forceinline__ void rebase(float& s, float& q, float from, float m, float k) {
+    const float d = fmaxf(from - scaled(m, k), -1e30f);
+    const float f = ex2_approx(d);
+    q = fmaf(s, d, q) * f;
+    s *= f;
 }
 
+template <bool ENT>
 __device__ __forceinline__ Part warp_part(const Acc& a, float k) {
     Part p;
     p.m = warp_max(a.mx);
-    float s = a.s, q = a.q;
-    // an untouched thread (ref NEG, sums 0) and one of only -inf end at 0
-    rebase(s, q, a.ref, p.m, k);
-    p.s = warp_sum((double)s);
-    p.q = warp_sum((double)q);
+    float s0, s1, q0, q1;
+    unpack2(a.s, s0, s1);
+    unpack2(a.q, q0, q1);
+    s0 += s1, q0 += q1;
+    rebase(s0, q0, a.c, p.m, k);
+    p.s = warp_sum(s0);
+    p.q = ENT ? warp_sum(q0) : 0.0f;
+    p.pad = 0.0f;
     return p;
 }
+
+// A row's joined sums: 2^(l * k - R) over the row adds to S.
+struct Row {
+    float M;
+    double S, Q, R;
+    bool wide;
+};
+
+// One warp joins n parts, in the same order in every warp.
+template <bool ENT>
+__device__ __forceinline__ Row join_parts(const Part* parts, int n, float k) {
+    const int lane = threadIdx.x & 31;
+    Row w;
+    w.M = -INFINITY;
+    for (int i = lane; i < n; i += 32) w.M = fmaxf(w.M, parts[i].m);
+    w.M = warp_max(w.M);
+    float s = 0.0f, q = 0.0f;
+    for (int i = lane; i < n; i += 32) {
+        Part p = parts[i];
+        rebase(p.s, p.q, scaled(p.m, k), w.M, k);
+        s += p.s, q += p.q;
+    }
+    w.S = warp_sum((double)s);
+    w.Q = ENT ? warp_sum((double)q) : 0.0;
+    const float c = scaled(w.M, k);
+    w.R = (double)c;
+    w.wide = fabsf(c) > WIDE && !isinf(w.M);
+    return w;
+}
+
+// ---- one row's scalars ------------------------------------------------------
+
+// grad_v = 2^(l * k - c) * (a + b * (l * k - c)) + [v == target] * one
+struct Coef {
+    float c, a, b, one;
+    float lt;  // the target's logit
+    int kind;  // ROW_*
+};
+enum { ROW_SUM = 0, ROW_ZERO = 1, ROW_NAN = 2, ROW_WIDE = 3 };  // ROW_WIDE: c is M itself, t = (l - c) * k
+
+// The gradient of g_lp * logprob + g_ent * entropy: p_v = 2^t / S and
+// ln p_v = ln2 * t - ln S, so (g_lp ([v==target] - p) - g_ent p (ln p + H)) / T
+// has the form of Coef, with H - ln S = -ln2 * Q / S. Where both derivatives
+// are 0 (a clipped ratio) the row's gradient is zeros, without its logits.
+__device__ __forceinline__ Coef make_coef(float M, float R, bool wide, float S, float h_ln_s, float g_lp, float g_ent, float inv_t) {
+    Coef o;
+    const float w = -inv_t / S;
+    o.c = wide ? M : R;
+    o.a = w * (g_lp + (g_ent != 0.0f ? g_ent * h_ln_s : 0.0f));
+    o.b = w * (float)LN2 * g_ent;
+    o.one = g_lp * inv_t;
+    o.lt = 0.0f;
+    o.kind = (g_lp == 0.0f && g_ent == 0.0f) ? ROW_ZERO : S != S ? ROW_NAN : M == -INFINITY ? ROW_ZERO : wide ? ROW_WIDE : ROW_SUM;
+    return o;
+}
+// A row without an element-wise gradient.
+__device__ __forceinline__ Coef fill_coef(bool nan) {
+    Coef o;
+    o.c = o.a = o.b = o.one = o.lt = 0.0f;
+    o.kind = nan ? ROW_NAN : ROW_ZERO;
+    return o;
+}
+
+struct RowIn {  // a row's inputs beside its logits
+    float lt, adv, old_lp, ref_lp;
+    double weight;
+};
+
+// ln S for S >= 1 (or 0, NaN) to about 1e-7 absolute: the exponent's part in
+// 64 bits, the mantissa's by logf on [1, 2).
+__device__ __forceinline__ double ln_sum(double S) {
+    const float s = (float)S;
+    const int e = ((__float_as_int(s) >> 23) & 255) - 127;
+    if (!(s > 1e-30f && s < 1e30f)) return (double)logf(s);
+    const float m = __int_as_float((__float_as_int(s) & 0x007FFFFF) | 0x3F800000);
+    // the rounding of S to s goes in to first order
+    return e * LN2 + (double)(logf(m) + (float)((S - (double)s)) / s);
+}
+
+// Writes a row's outputs (one thread) and returns its gradient's
+// coefficients. The log-probability is formed in 64 bits; the exponentials of
+// its differences, which are near 1, are expf's (2^-23 relative): their
+// 64-bit forms took 1.4 us on the path between the row's two passes.
+template <bool ENT, bool POLICY>
+__device__ __forceinline__ Coef finish_row(const Args& a, int64_t r, const Row& w, const RowIn& in, bool write) {
+    const bool none = w.M == -INFINITY && w.S == 0.0;
+    const double lnS = ln_sum(w.S);
+    const double lp = none ? -INFINITY : ((double)in.lt * (double)a.k - w.R) * LN2 - lnS;
+    const float S = (float)w.S;
+    const float h_ln_s = ENT && !none ? (float)-LN2 * ((float)w.Q / S) : 0.0f;
+    const float H = ENT && !none ? (float)(lnS + (double)h_ln_s) : 0.0f;
+    float loss = 0.0f;
+    Coef c = fill_coef(false);
+    if (POLICY) {
+        const float adv = in.adv, ratio = expf((float)(lp - (double)in.old_lp));
+        const float lo = (float)(1.0 - a.clip_lo), hi = (float)(1.0 + a.clip_hi);
+        const float fit = ratio < lo ? lo : ratio > hi ? hi : ratio;  // NaN stays
+        const float x = ratio * adv, y = fit * adv;
+        loss = x <= y ? -x : y < x ? -y : NAN;
+        float g = x <= y ? -x : y < x ? 0.0f : NAN;
+        if (a.kl != 0.0) {
+            const float u = (float)((double)in.ref_lp - lp), eu = expm1f(u);
+            loss += (float)a.kl * (eu - u);
+            g -= (float)a.kl * eu;
+        }
+        if (ENT && a.ec != 0.0) loss -= (float)a.ec * H;
+        g *= (float)(in.weight * a.scale);
+        if (a.grad) c = make_coef(w.M, (float)w.R, w.wide, S, h_ln_s, g, ENT ? (float)(-a.ec * in.weight * a.scale) : 0.0f, (float)a.inv_t);
+        c.lt = in.lt;
+    }
+    if (write) {
+        a.logprob[r] = (float)lp;
+        if (a.entropy) a.entropy[r] = H;
+        // S was summed against R, the rounded M * k
+        if (a.stats) a.stats[r] = {w.M, S * (none ? 1.0f : ex2_approx((float)(w.R - (double)w.M * (double)a.k)))};
+        if (a.row_grad) a.row_grad[r] = 0.0f;
+        if (POLICY) a.row_loss[r] = loss;
+    }
+    return c;
+}
+
+// Outputs of a row that takes no part (0) or whose target is out of range (NaN).
+template <bool POLICY>
+__device__ __forceinline__ void blank_row(const Args& a, int64_t r, float v) {
+    a.logprob[r] = v;
+    if (a.entropy) a.entropy[r] = v;
+    if (a.stats) a.stats[r] = {0.0f, 0.0f};
+    if (a.row_grad) a.row_grad[r] = 0.0f;
+    if (POLICY) a.row_loss[r] = v;
+}
+
+// ---- the gradient ------------------------------------------------------------
+
+template <bool ENT>
+__device__ __forceinline__ float grad1(const Coef& c, float l, float k) {
+    const float t = c.kind == ROW_WIDE ? (l - c.c) * k : fmaf(l, k, -c.c);
+    const float e = ex2_approx(t);
+    return ENT ? e * fmaf(c.b, fmaxf(t, -200.0f), c.a) : e * c.a;
+}
+
+// A pack's gradient (rows of ROW_SUM).
+template <bool ENT, int N>
+__device__ __forceinline__ void grad_pack(float (&x)[N], const Coef& c, float k) {
+    const f32x2 nc = pack2(-c.c, -c.c), kk = pack2(k, k), aa = pack2(c.a, c.a), bb = pack2(c.b, c.b);
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+        const f32x2 t = fma2(pack2(x[i], x[i + 1]), kk, nc);
+        float t0, t1;
+        unpack2(t, t0, t1);
+        f32x2 e = pack2(ex2_approx(t0), ex2_approx(t1));
+        e = mul2(e, ENT ? fma2(bb, pack2(fmaxf(t0, -200.0f), fmaxf(t1, -200.0f)), aa) : aa);
+        unpack2(e, x[i], x[i + 1]);
+    }
+}
+
+template <typename T, bool ENT>
+__device__ __forceinline__ uint4 grad_of(const uint4& p, const Coef& c, float k) {
+    float x[Type<T>::N];
+    widen(p, x, (T*)nullptr);
+    grad_pack<ENT>(x, c, k);
+    return narrow(x, (T*)nullptr);
+}
+
+// The same for rows of ROW_WIDE (rare: out of the streaming loops).
+template <typename T, bool ENT>
+__device__ __noinline__ uint4 grad_of_wide(uint4 p, Coef c, float k) {
+    float x[Type<T>::N];
+    widen(p, x, (T*)nullptr);
+#pragma unroll
+    for (int i = 0; i < Type<T>::N; i++) x[i] = grad1<ENT>(c, x[i], k);
+    return narrow(x, (T*)nullptr);
+}
+
+__device__ __forceinline__ bool elementwise(const Coef& c) { return c.kind == ROW_SUM || c.kind == ROW_WIDE; }
+
+// A pack of zeros, or of NaN.
+template <typename T>
+__device__ __forceinline__ uint4 fill_pack(const Coef& c) {
+    float x[Type<T>::N];
+#pragma unroll
+    for (int i = 0; i < Type<T>::N; i++) x[i] = c.kind == ROW_NAN ? NAN : 0.0f;
+    return narrow(x, (T*)nullptr);
+}
+
+// Stores a pack whose place is not 16-byte aligned.
+template <typename T>
+__device__ __noinline__ void store_elements(T* dst, uint4 p) {
+    const uint32_t w[4] = {p.x, p.y, p.z, p.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if (sizeof(T) == 4) {
+            reinterpret_cast<uint32_t*>(dst)[i] = w[i];
+        } else {
+            reinterpret_cast<uint16_t*>(dst)[2 * i] = (uint16_t)w[i];
+            reinterpret_cast<uint16_t*>(dst)[2 * i + 1] = (uint16_t)(w[i] >> 16);
+        }
+    }
+}
+
+// An edge element's gradient.
+template <typename T, bool ENT>
+__device__ __forceinline__ void put_edge(T* out, int v, int target, float l, const Coef& c, float k) {
+    put1(out + v, c.kind == ROW_ZERO ? 0.0f : c.kind == ROW_NAN ? NAN : grad1<ENT>(c, l, k) + (v == target ? c.one : 0.0f));
+}
+
+// Writes a row's gradient where no batch loop fits: element-wise gradients of
+// wide rows, fills, and rows of another 16-byte phase than the logits'.
+// Packs [lo, hi), pack lo + i by thread i % nt.
+template <typename T, bool ENT>
+__device__ __noinline__ void grad_plain(const T* row, T* out, int head, int lo, int hi, Coef c, float k, int nt) {
+    const uint4* src = reinterpret_cast<const uint4*>(row + head);
+    T* dst = out + head;
+    const bool same = ((uintptr_t)dst & 15) == 0;
+    const uint4 fill = fill_pack<T>(c);
+#pragma unroll 4
+    for (int v = lo + (int)threadIdx.x; v < hi; v += nt) {
+        uint4 g = fill;
+        if (elementwise(c)) {
+            const uint4 p = load_pack(src + v);
+            g = c.kind == ROW_SUM ? grad_of<T, ENT>(p, c, k) : grad_of_wide<T, ENT>(p, c, k);
+        }
+        if (same)
+            reinterpret_cast<uint4*>(dst)[v] = g;
+        else
+            store_elements(dst + (int64_t)v * Type<T>::N, g);
+    }
+}
+
+// ---- clusters ----------------------------------------------------------------
 
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
@@ -192,219 +507,608 @@ __device__ __forceinline__ uint32_t cluster_size() {
 }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-__device__ __forceinline__ void remote_store(const void* local, uint32_t rank, const Part& p) {
-    const uint32_t a = (uint32_t)__cvta_generic_to_shared(local);
+__device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
     uint32_t r;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
-    asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(r), "d"(p.s) : "memory");
-    asm volatile("st.shared::cluster.f64 [%0+8], %1;" ::"r"(r), "d"(p.q) : "memory");
-    asm volatile("st.shared::cluster.f32 [%0+16], %1;" ::"r"(r), "f"(p.m) : "memory");
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void remote_store(uint32_t addr, const Part& p) {
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "f"(p.m), "f"(p.s), "f"(p.q), "f"(p.pad) : "memory");
 }
 
-// ---- the gradient of one slice ---------------------------------------------
+// Sums of one thread's share of a slice against M itself, with differences
+// taken before the multiply: for rows whose maximum is so large, or so low,
+// that l * k overflows (a row masked throughout by the type's lowest value).
+template <typename T, bool ENT>
+__device__ __noinline__ Part wide_part(const T* row, int V, float M, float k, int part, int parts, int first, int nt) {
+    const Slice sl = slice_of(row, V, part, parts);
+    const int v0 = part == 0 ? 0 : sl.head + sl.lo * Type<T>::N, v1 = part == parts - 1 ? V : sl.head + (sl.lo + sl.n) * Type<T>::N;
+    float s = 0.0f, q = 0.0f;
+#pragma unroll 4
+    for (int v = v0 + first; v < v1; v += nt) {
+        const float t = (widen1(row[v]) - M) * k;
+        const float e = ex2_approx(t);
+        s += e;
+        if (ENT) q = fmaf(e, fmaxf(t, -200.0f), q);
+    }
+    return Part{M, warp_sum(s), ENT ? warp_sum(q) : 0.0f, 0.0f};
+}
 
-// grad_v = 2^(d*k) * (a + b * d*k) + [v == target] * one
-struct Coef {
-    float m, a, b, one;
-    int kind;  // 0 as above, 1 zeros, 2 NaN
+// Joins such parts.
+__device__ __forceinline__ Row join_wide(const Part* parts, int n, float M, float k) {
+    const int lane = threadIdx.x & 31;
+    Row w;
+    double s = 0.0, q = 0.0;
+    for (int i = lane; i < n; i += 32) s += (double)parts[i].s, q += (double)parts[i].q;
+    w.M = M;
+    w.S = warp_sum(s), w.Q = warp_sum(q);
+    w.R = (double)M * (double)k;
+    w.wide = true;
+    return w;
+}
+
+// Lets a kernel launched behind this one with programmatic serialization start
+// (it waits for this one's end before it reads).
+__device__ __forceinline__ void launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// ---- a cluster per row ---------------------------------------------------------
+
+// Log-probabilities, and the policy loss of few or of short rows: one cluster
+// (or one CTA) per row, each CTA a slice of it. The sums come from memory; for
+// the gradient the slice is read again, from L2 (or not at all: the last
+// batch of packs is still in registers, which is all of a short slice).
+// Measured at V = 151936: 8191 bf16 rows, a tenth of them left out, in 325 us
+// (1.05 of the measured copy rate: reads are a little faster than copies); one fp32
+// row in 6.2 us.
+template <typename T, bool ENT, bool POLICY, int NT>
+__global__ void __launch_bounds__(NT, 1024 / NT) rows_kernel(const Args a) {
+    constexpr int N = Type<T>::N, NW = NT / 32, STEP = NT * U;
+    __shared__ Part parts[2][MAXC * NW];
+    __shared__ Coef coef;
+    __shared__ bool again;
+    __shared__ float wide_m;
+    const int C = (int)cluster_size(), rank = (int)cluster_rank();
+    const int64_t r = blockIdx.x / C;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const T* row = (const T*)a.logits + r * a.ld;
+    const float k = a.k;
+    const int target = a.targets[r];
+    const double weight = POLICY ? (a.weight ? (double)a.weight[r] : a.mean) : 1.0;
+    const Slice s = slice_of(row, a.V, rank, C);
+    const uint4* src = reinterpret_cast<const uint4*>(row + s.head) + s.lo + tid;
+    // the first batch is the ragged one, and on its way before the row is known to take part
+    int first = s.n % STEP;
+    if (first == 0) first = min(s.n, STEP);
+    uint4 p[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        p[u] = make_uint4(Type<T>::NEG_INF, Type<T>::NEG_INF, Type<T>::NEG_INF, Type<T>::NEG_INF);
+        if (u * NT + tid < first) p[u] = load_pack(src + u * NT);
+    }
+    if (C > 1) cluster_arrive();  // the peers' shared memory is written below
+
+    const bool live = target >= 0 && weight != 0.0, bad = target >= a.V;
+    T* out = (T*)a.grad + r * a.grad_ld;
+    if (!live || bad) {
+        if (C > 1) cluster_wait();
+        launch_next();
+        if (rank == 0 && tid == 0) blank_row<POLICY>(a, r, live ? NAN : 0.0f);
+        if (POLICY && a.grad) {
+            const Coef c = fill_coef(live);
+            if (s.edge >= 0) put_edge<T, ENT>(out, s.edge, target, 0.0f, c, k);
+            grad_plain<T, ENT>(row, out, s.head, s.lo, s.lo + s.n, c, k, NT);
+        }
+        return;
+    }
+    RowIn in{0.0f, 0.0f, 0.0f, 0.0f, weight};
+    if (warp == 0) {
+        in.lt = widen1(row[target]);
+        if (POLICY) {
+            in.adv = a.adv[r], in.old_lp = a.old_lp[r];
+            if (a.kl != 0.0) in.ref_lp = a.ref_lp[r];
+        }
+    }
+    const float edge = s.edge >= 0 ? widen1(row[s.edge]) : -INFINITY;
+    Acc acc = acc_new();
+    int held = 0;  // the batch in p
+    for (int v = first; v < s.n; v += STEP) {
+        acc_packs<T, ENT>(acc, p, k);
+#pragma unroll
+        for (int u = 0; u < U; u++) p[u] = load_pack(src + v + u * NT);
+        held = v;
+    }
+    acc_packs<T, ENT>(acc, p, k);
+    if (s.edge >= 0) acc_one<ENT>(acc, edge, k);
+    Part mine = warp_part<ENT>(acc, k);
+    float wide = 0.0f;  // M of a wide row in its second turn
+    for (int turn = 0; turn < 2; turn++) {
+        if (C > 1) {
+            if (turn == 0) cluster_wait();  // the peers run
+            if (lane < C) remote_store(map_rank(smem_u32(&parts[turn][rank * NW + warp]), lane), mine);
+            cluster_arrive();
+            cluster_wait();
+        } else {
+            if (lane == 0) parts[turn][warp] = mine;
+            __syncthreads();
+        }
+        if (warp == 0) {
+            const Row w = turn ? join_wide(parts[1], C * NW, wide, k) : join_parts<ENT>(parts[0], C * NW, k);
+            Coef c = fill_coef(false);
+            if (turn || !w.wide) c = finish_row<ENT, POLICY>(a, r, w, in, rank == 0 && lane == 0);
+            if (lane == 0) coef = c, again = !turn && w.wide, wide_m = w.M;
+        }
+        __syncthreads();
+        if (!again) break;
+        wide = wide_m;
+        mine = wide_part<T, ENT>(row, a.V, wide, k, rank, C, tid, NT);
+        __syncthreads();  // again and wide_m are written once more
+    }
+    launch_next();
+    if (!POLICY || !a.grad) return;
+
+    const Coef c = coef;
+    if (s.edge >= 0) put_edge<T, ENT>(out, s.edge, target, edge, c, k);
+    T* dst = out + s.head + (int64_t)(s.lo + tid) * N;
+    const int hot = target >= s.head ? (target - s.head) / N - s.lo : -1;  // the target's pack, if 0 <= hot < s.n
+    int hot_thread = hot % NT;
+    if (((uintptr_t)dst & 15) == 0 && c.kind == ROW_SUM) {
+        uint4* d = reinterpret_cast<uint4*>(dst);
+        const int end = held ? s.n : first;
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (held + u * NT + tid < end) __stcs(d + held + u * NT, (grad_of<T, ENT>(p[u], c, k)));
+        for (int v = held - STEP; v >= first; v -= STEP) {
+#pragma unroll
+            for (int u = 0; u < U; u++) p[u] = load_pack(src + v + u * NT);
+#pragma unroll
+            for (int u = 0; u < U; u++) __stcs(d + v + u * NT, (grad_of<T, ENT>(p[u], c, k)));
+        }
+        if (held) {
+#pragma unroll
+            for (int u = 0; u < U; u++)
+                if (u * NT + tid < first) p[u] = load_pack(src + u * NT);
+#pragma unroll
+            for (int u = 0; u < U; u++)
+                if (u * NT + tid < first) __stcs(d + u * NT, (grad_of<T, ENT>(p[u], c, k)));
+        }
+        if (hot >= first) hot_thread = (hot - first) % NT;  // batches begin at first + i * STEP
+    } else {
+        grad_plain<T, ENT>(row, out, s.head, s.lo, s.lo + s.n, c, k, NT);
+    }
+    // the thread that wrote the target's pack puts the target right
+    if (hot >= 0 && hot < s.n && tid == hot_thread && elementwise(c)) put1(out + target, grad1<ENT>(c, c.lt, k) + c.one);
+}
+
+// ---- a stream of rows per cluster ----------------------------------------------
+
+// The policy loss with its gradient over many long rows. Persistent clusters,
+// each CTA a slice of every row of its cluster; a producer warp streams the
+// slices through a ring of chunks in shared memory (bulk copies), a joining
+// warp turns sums into coefficients, and NT consumer threads work on chunks in
+// this order, the same in producer and consumers: chunks of row i for its
+// sums, and behind the first LAG_CHUNKS of them, in turn with the others, the
+// chunks of the row before for its gradient, read again from L2. So a row's
+// sums travel to the joining warp and back while the consumers are busy, and
+// loads of one row stand beside stores of another.
+//
+// The rows in flight have to stay in L2 between their two readings: the
+// launcher takes the cluster size that keeps them under STREAM_L2 bytes.
+// Rows that take no part are left out of the stream (a bit per row in shared
+// memory), so that every cluster gets the same number of live rows, and are
+// filled at the end.
+constexpr int LAG_CHUNKS = 1;
+constexpr int STREAM_ROWS = 16384;  // rows of one launch at most
+
+template <int NT_, int CTAS_, int PP_, int STAGES_>
+struct StreamShape {
+    static constexpr int NT = NT_;          // consumer threads
+    static constexpr int CTAS = CTAS_;      // CTAs per SM
+    static constexpr int PP = PP_;          // packs of a thread per chunk
+    static constexpr int STAGES = STAGES_;  // chunks of the ring
+    static constexpr int NW = NT / 32, CHP = NT * PP, CH = CHP * 16;
 };
 
-// p_v = 2^t / S with t = d*k, ln p_v = ln2 * (t - log2 S), so
-// (g_lp ([v==target] - p) - g_ent p (ln p + H)) / T has this form.
-__device__ __forceinline__ Coef make_coef(double M, double S, double H, double g_lp, double g_ent, double inv_t) {
-    Coef c;
-    const double w = -inv_t / S;
-    c.m = (float)M;
-    c.a = (float)(w * (g_lp + (g_ent != 0.0 ? g_ent * (H - log(S)) : 0.0)));
-    c.b = (float)(w * LN2 * g_ent);
-    c.one = (float)(g_lp * inv_t);
-    c.kind = S != S ? 2 : M == -INFINITY ? 1 : 0;
-    return c;
+template <typename Shape>
+struct StreamShared {
+    Part own[2][Shape::NW];   // of the rows in turn, from the CTA's warps
+    Part parts[2][MAXC];      // ... and from the cluster's CTAs
+    Part wide_parts[MAXC];
+    uint64_t full[Shape::STAGES], empty[Shape::STAGES];
+    uint64_t obar[2], xbar[2], cbar[2], wbar;  // own parts, parts, coefficients, wide parts are here
+    Coef coef[2];
+    int rows[8];              // the rows whose first chunks are out, in turn
+    uint32_t live[STREAM_ROWS / 32], before[STREAM_ROWS / 32];  // rows that take part; their number before each word
+    int nlive;
+    int abort;
+};
+
+// Stores p at a peer's shared address; the peer's barrier counts the bytes.
+__device__ __forceinline__ void send_part(uint32_t addr, uint32_t bar, const Part& p) {
+    asm volatile(
+        "st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1,%2,%3,%4}, [%5];" ::"r"(addr), "f"(p.m),
+        "f"(p.s), "f"(p.q), "f"(p.pad), "r"(bar)
+        : "memory");
 }
 
-template <bool ENT>
-__device__ __forceinline__ float grad1(const Coef& c, float l, float k) {
-    const float t = (l - c.m) * k;
-    const float e = ex2_approx(t);
-    return ENT ? e * fmaf(c.b, fmaxf(t, -200.0f), c.a) : e * c.a;
-}
-
-// Writes CTA `part` of `parts`' share of a row's gradient.
-template <typename T, bool ENT>
-__device__ __forceinline__ void grad_slice(const T* row, T* out, int V, int target, const Coef& c, float k, int part, int parts) {
-    constexpr int N = Type<T>::N;
-    const Span sp = span_of(row, V);
-    const int tid = threadIdx.x;
-    const float fill = c.kind == 2 ? NAN : 0.0f;
-    if (part == 0 && tid < sp.head + sp.tail) {
-        const int v = tid < sp.head ? tid : V - sp.tail + (tid - sp.head);
-        put1(out + v, c.kind ? fill : grad1<ENT>(c, widen1(row[v]), k) + (v == target ? c.one : 0.0f));
+// Waits for a phase of `bar`. After WAIT_CYCLES, or once another wait of the
+// CTA has given up, returns all the same: the CTA's rows then come out NaN.
+__device__ __forceinline__ void stream_wait(uint32_t bar, uint32_t parity, volatile int* abort) {
+    if (mbar_try_wait(bar, parity)) return;
+    const long long t0 = clock64();
+    while (!mbar_try_wait(bar, parity)) {
+        if (*abort) return;
+        if (clock64() - t0 > WAIT_CYCLES) {
+            *abort = 1;
+            return;
+        }
     }
-    const int lo = (int)((int64_t)sp.packs * part / parts), hi = (int)((int64_t)sp.packs * (part + 1) / parts);
-    const uint4* src = reinterpret_cast<const uint4*>(row + sp.head);
-    T* dst = out + sp.head;
-    const bool same = ((uintptr_t)dst & 15) == 0;
-    const int hot = target >= sp.head ? (target - sp.head) / N : -1;  // the target's pack (tail: none here)
-    for (int v0 = lo + tid; v0 < hi; v0 += NT * U) {
+}
+
+__device__ __forceinline__ uint4 lds_pack(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+    return v;
+}
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar, uint64_t pol) {
+    asm volatile(
+        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;" ::"r"(dst),
+        "l"(src), "r"(bytes), "r"(bar), "l"(pol)
+        : "memory");
+}
+
+// The j-th row (from 0) that takes part, or with dead that does not.
+template <typename Shape>
+__device__ __forceinline__ int64_t nth_row(const StreamShared<Shape>& sh, int rows, int j, bool dead) {
+    int lo = 0, hi = (rows + 31) / 32;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2, n = (int)sh.before[mid];
+        if ((dead ? 32 * mid - n : n) <= j)
+            lo = mid;
+        else
+            hi = mid;
+    }
+    uint32_t m = dead ? ~sh.live[lo] : sh.live[lo];
+    j -= dead ? 32 * lo - (int)sh.before[lo] : (int)sh.before[lo];
+    for (; j > 0; j--) m &= m - 1;
+    return 32 * lo + __ffs(m) - 1;
+}
+
+template <typename T, bool ENT, typename Shape>
+__global__ void __launch_bounds__(Shape::NT + 64, Shape::CTAS) stream_kernel(const Args a) {
+    constexpr int N = Type<T>::N, NT = Shape::NT, NW = Shape::NW, PP = Shape::PP, CHP = Shape::CHP, CH = Shape::CH;
+    constexpr uint32_t STAGES = Shape::STAGES;
+    extern __shared__ __align__(128) unsigned char ring[];
+    __shared__ StreamShared<Shape> sh;
+    const int C = (int)cluster_size(), rank = (int)cluster_rank();
+    const int cid = (int)(blockIdx.x / C), step = (int)(gridDim.x / C);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const uint32_t ring_u = smem_u32(ring), full_u = smem_u32(sh.full), empty_u = smem_u32(sh.empty);
+    const uint32_t obar_u = smem_u32(sh.obar), xbar_u = smem_u32(sh.xbar), cbar_u = smem_u32(sh.cbar), wbar_u = smem_u32(&sh.wbar);
+    volatile int* abort = &sh.abort;
+    const float k = a.k;
+
+    if (tid == 0) {
+        for (uint32_t i = 0; i < STAGES; i++) {
+            mbar_init(full_u + 8 * i, 1);
+            mbar_init(empty_u + 8 * i, NW);
+        }
+        for (int i = 0; i < 2; i++) {
+            mbar_init(obar_u + 8 * i, NW);
+            mbar_init(xbar_u + 8 * i, 1);
+            mbar_init(cbar_u + 8 * i, 1);
+        }
+        mbar_init(wbar_u, 1);
+        sh.abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    const int words = (a.rows + 31) / 32;
+    for (int w = warp; w < words; w += NW + 2) {
+        const int r = 32 * w + lane, t = r < a.rows ? a.targets[r] : -1;
+        const unsigned m = __ballot_sync(FULL, t >= 0 && t < a.V && !(a.weight && a.weight[r] == 0.0f));
+        if (lane == 0) sh.live[w] = m;
+    }
+    __syncthreads();
+    if (warp == 0) {
+        int sum = 0;
+        for (int w0 = 0; w0 < words; w0 += 32) {
+            const int n = w0 + lane < words ? __popc(sh.live[w0 + lane]) : 0, upto = warp_incl_scan(n, lane);
+            if (w0 + lane < words) sh.before[w0 + lane] = (uint32_t)(sum + upto - n);
+            sum += __shfl_sync(FULL, upto, 31);
+        }
+        if (lane == 0) sh.nlive = sum;
+    }
+    __syncthreads();
+    cluster_arrive();
+    cluster_wait();
+    const int mine_n = sh.nlive > cid ? (sh.nlive - cid + step - 1) / step : 0;  // rows of this cluster
+
+    if (warp == NW) {  // ---- the producer warp: its first lane issues the copies
+        if (lane == 0) {
+            uint64_t again, once;
+            asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(again));
+            asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(once));
+            uint32_t stage = 0, phase = 0, issued = 0;
+            const uint4* b_src = nullptr;  // the row before, whose gradient is due
+            int b_n = 0, b_packs = 0;
+            const auto put = [&](const uint4* src, int j, int packs, uint64_t pol) {
+                const uint32_t bytes = (uint32_t)min(CHP, packs - j * CHP) * 16;
+                stream_wait(empty_u + 8 * stage, phase ^ 1, abort);
+                if (*abort) return;
+                mbar_arrive_tx(full_u + 8 * stage, bytes);
+                bulk_load(ring_u + stage * CH, src + j * CHP, bytes, full_u + 8 * stage, pol);
+                issued++;
+                if (++stage == STAGES) stage = 0, phase ^= 1;
+            };
+            for (int i = 0; i <= mine_n && !*abort; i++) {
+                const uint4* src = nullptr;
+                int n = 0, packs = 0;
+                if (i < mine_n) {
+                    const int64_t r = nth_row(sh, a.rows, cid + i * step, false);
+                    const T* row = (const T*)a.logits + r * a.ld;
+                    const Slice s = slice_of(row, a.V, rank, C);
+                    src = reinterpret_cast<const uint4*>(row + s.head) + s.lo;
+                    packs = s.n, n = (s.n + CHP - 1) / CHP;
+                    sh.rows[i & 7] = (int)r;
+                }
+                const int lag = min(n, LAG_CHUNKS), steps = max(n, lag + b_n);
+                for (int j = 0; j < steps && !*abort; j++) {
+                    if (j < n) put(src, j, packs, again);
+                    if (j >= lag && j - lag < b_n) put(b_src, j - lag, b_packs, once);
+                }
+                b_src = src, b_n = n, b_packs = packs;
+            }
+            if (*abort) {  // let the copies in flight land
+                const uint32_t n = min(issued, STAGES);
+                for (uint32_t i = 0; i < n; i++) {
+                    if (stage == 0) stage = STAGES, phase ^= 1;
+                    stage--;
+                    mbar_wait(full_u + 8 * stage, phase);
+                }
+            }
+        }
+    } else if (warp == NW + 1) {  // ---- the joining warp: sums to coefficients
+        uint32_t phases = 0;  // of xbar and obar, a bit for each parity
+        uint32_t wphase = 0;
+        const auto inputs = [&](int64_t r) {
+            RowIn in{0.0f, 0.0f, 0.0f, 0.0f, 0.0};
+            in.lt = widen1(((const T*)a.logits + r * a.ld)[a.targets[r]]);
+            in.adv = a.adv[r], in.old_lp = a.old_lp[r];
+            if (a.kl != 0.0) in.ref_lp = a.ref_lp[r];
+            in.weight = a.weight ? (double)a.weight[r] : a.mean;
+            return in;
+        };
+        int64_t next = mine_n ? nth_row(sh, a.rows, cid, false) : 0;
+        RowIn next_in = mine_n ? inputs(next) : RowIn{};
+        for (int i = 0; i < mine_n; i++) {
+            const int par = i & 1;
+            const int64_t r = next;
+            const RowIn in = next_in;
+            // the next row's target is read before this row's coefficients are
+            // out: behind them a peer may come to write over the next row
+            if (i + 1 < mine_n) {
+                next = nth_row(sh, a.rows, cid + (i + 1) * step, false);
+                next_in = inputs(next);
+            }
+            stream_wait(obar_u + 8 * par, (phases >> par) & 1, abort);
+            Row w = join_parts<ENT>(sh.own[par], NW, k);
+            if (C > 1) {
+                if (lane == 0) mbar_arrive_tx(xbar_u + 8 * par, C * 16);
+                __syncwarp();
+                if (lane < C && !*abort)
+                    send_part(map_rank(smem_u32(&sh.parts[par][rank]), lane), map_rank(xbar_u + 8 * par, lane), Part{w.M, (float)w.S, (float)w.Q, 0.0f});
+                stream_wait(xbar_u + 8 * par, (phases >> par) & 1, abort);
+                w = join_parts<ENT>(sh.parts[par], C, k);
+            }
+            phases ^= 1u << par;
+            if (*abort) w.S = NAN, w.wide = false;
+            if (w.wide) {  // the same in every CTA: once more through the slices, by these warps
+                const T* row = (const T*)a.logits + r * a.ld;
+                const Part own = wide_part<T, ENT>(row, a.V, w.M, k, rank, C, lane, 32);
+                if (lane == 0) mbar_arrive_tx(wbar_u, C * 16);
+                __syncwarp();
+                if (lane < C && !*abort) send_part(map_rank(smem_u32(&sh.wide_parts[rank]), lane), map_rank(wbar_u, lane), own);
+                stream_wait(wbar_u, wphase, abort);
+                wphase ^= 1;
+                w = join_wide(sh.wide_parts, C, w.M, k);
+                if (*abort) w.S = NAN;
+            }
+            const Coef c = finish_row<ENT, true>(a, r, w, in, rank == 0 && lane == 0);
+            if (lane == 0) {
+                sh.coef[par] = c;
+                mbar_arrive(cbar_u + 8 * par);
+            }
+            __syncwarp();
+        }
+    } else {  // ---- the consumers
+        uint32_t stage = 0, phase = 0, cphase = 0;
+        // the row before, whose gradient is due
+        T* b_out = nullptr;
+        Slice b{};
+        int b_n = 0;
+        float b_edge = 0.0f;
+        int b_target = -1;
+        for (int i = 0; i <= mine_n; i++) {
+            const int par = i & 1;
+            const bool more = i < mine_n;
+            Slice s{};
+            s.edge = -1;
+            const T* row = nullptr;
+            int64_t r = 0;
+            float edge = -INFINITY;
+            int n = 0;
+            if (more) {  // the row's number comes with its first chunk
+                stream_wait(full_u + 8 * stage, phase, abort);
+                r = *abort ? nth_row(sh, a.rows, cid + i * step, false) : *(volatile int*)&sh.rows[i & 7];
+                row = (const T*)a.logits + r * a.ld;
+                s = slice_of(row, a.V, rank, C);
+                n = (s.n + CHP - 1) / CHP;
+                if (s.edge >= 0) edge = widen1(row[s.edge]);
+            }
+            const int lag = min(n, LAG_CHUNKS), steps = max(more ? n + 1 : 0, lag + b_n);
+            Acc acc = acc_new();
+            Coef c;
+            bool have_c = i == 0;
+            T* b_dst = b_out + b.head + (int64_t)b.lo * N;
+            const bool same = ((uintptr_t)b_dst & 15) == 0;
+            const auto want_c = [&]() {  // the coefficients of the row before
+                if (have_c) return;
+                stream_wait(cbar_u + 8 * (par ^ 1), (cphase >> (par ^ 1)) & 1, abort);
+                cphase ^= 1u << (par ^ 1);
+                c = sh.coef[par ^ 1];
+                if (*abort) c.kind = ROW_NAN;
+                have_c = true;
+            };
+            for (int j = 0; j < steps; j++) {
+                if (j < n) {
+                    stream_wait(full_u + 8 * stage, phase, abort);
+                    const uint32_t at = ring_u + stage * CH + tid * 16;
+                    uint4 p[PP];
+                    if (j + 1 < n) {
+#pragma unroll
+                        for (int u = 0; u < PP; u++) p[u] = lds_pack(at + u * NT * 16);
+                    } else {
+#pragma unroll
+                        for (int u = 0; u < PP; u++) {
+                            p[u] = make_uint4(Type<T>::NEG_INF, Type<T>::NEG_INF, Type<T>::NEG_INF, Type<T>::NEG_INF);
+                            if (j * CHP + u * NT + tid < s.n) p[u] = lds_pack(at + u * NT * 16);
+                        }
+                    }
+                    acc_packs<T, ENT>(acc, p, k);
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(empty_u + 8 * stage);
+                    if (++stage == STAGES) stage = 0, phase ^= 1;
+                } else if (j == n && more) {
+                    if (s.edge >= 0) acc_one<ENT>(acc, edge, k);
+                    const Part mine = warp_part<ENT>(acc, k);
+                    // two buffers in turn: a warp hands in row i + 1 only with row i's coefficients in hand
+                    want_c();
+                    if (lane == 0) {
+                        sh.own[par][warp] = mine;
+                        mbar_arrive(obar_u + 8 * par);
+                    }
+                    __syncwarp();
+                }
+                if (j >= lag && j - lag < b_n) {
+                    want_c();
+                    const int base = (j - lag) * CHP + tid;
+                    stream_wait(full_u + 8 * stage, phase, abort);
+                    const uint32_t at = ring_u + stage * CH + tid * 16;
+                    uint4* d = reinterpret_cast<uint4*>(b_dst) + base;
+                    if (same && c.kind == ROW_SUM && j - lag + 1 < b_n) {
+#pragma unroll
+                        for (int u = 0; u < PP; u++) __stcs(d + u * NT, (grad_of<T, ENT>(lds_pack(at + u * NT * 16), c, k)));
+                    } else {
+#pragma unroll 1
+                        for (int u = 0; u < PP; u++)
+                            if (base + u * NT < b.n) {
+                                const uint4 p = lds_pack(at + u * NT * 16);
+                                const uint4 g = c.kind == ROW_SUM ? grad_of<T, ENT>(p, c, k) : c.kind == ROW_WIDE ? grad_of_wide<T, ENT>(p, c, k) : fill_pack<T>(c);
+                                if (same)
+                                    __stcs(d + u * NT, g);
+                                else
+                                    store_elements(b_dst + (int64_t)(base + u * NT) * N, g);
+                            }
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(empty_u + 8 * stage);
+                    if (++stage == STAGES) stage = 0, phase ^= 1;
+                }
+            }
+            if (i > 0) {
+                want_c();
+                if (b.edge >= 0) put_edge<T, ENT>(b_out, b.edge, b_target, b_edge, c, k);
+                // the thread that wrote the target's pack puts the target right
+                const int hot = b_target >= b.head ? (b_target - b.head) / N - b.lo : -1;
+                if (hot >= 0 && hot < b.n && hot % NT == tid && elementwise(c)) put1(b_out + b_target, grad1<ENT>(c, c.lt, k) + c.one);
+            }
+            if (more) {
+                b_out = (T*)a.grad + r * a.grad_ld;
+                b = s, b_n = n, b_edge = edge, b_target = a.targets[r];
+            }
+        }
+        // rows that take no part: zeros, or NaN for a target out of range
+        for (int j = (int)blockIdx.x; j < a.rows - sh.nlive; j += (int)gridDim.x) {
+            const int64_t r = nth_row(sh, a.rows, j, true);
+            const int target = a.targets[r];
+            const bool nan = target >= a.V && !(a.weight && a.weight[r] == 0.0f);
+            if (tid == 0) blank_row<true>(a, r, nan ? NAN : 0.0f);
+            const T* row = (const T*)a.logits + r * a.ld;
+            T* out = (T*)a.grad + r * a.grad_ld;
+            const Slice s = slice_of(row, a.V, 0, 1);
+            const Coef c = fill_coef(nan);
+            if (s.edge >= 0) put_edge<T, ENT>(out, s.edge, target, 0.0f, c, k);
+            grad_plain<T, ENT>(row, out, s.head, 0, s.n, c, k, NT);
+        }
+    }
+    // no CTA leaves while a peer may still store into its shared memory
+    __syncwarp();
+    launch_next();
+    cluster_arrive();
+    cluster_wait();
+}
+
+// ---- the gradient from given sums -------------------------------------------------
+
+// One CTA per slice of a row, `parts` of them in turn: one read and one write.
+// Measured: 2047 bf16 rows of 151936, a fifth of them zeros, in 177 us (0.97
+// of the measured copy rate) with slices of 76 KB; slices of a quarter of
+// that, in which a CTA's start weighs more, take 234 us.
+template <typename T, bool ENT>
+__global__ void __launch_bounds__(256, 6) grad_kernel(const Args a, const int parts) {
+    constexpr int N = Type<T>::N, NT = 256;
+    wait_before();
+    const int64_t r = blockIdx.x / (unsigned)parts;
+    const int part = (int)(blockIdx.x - (unsigned)r * (unsigned)parts);
+    const float k = a.k;
+    const int target = a.targets[r];
+    const float g_lp = a.g_lp[r], g_ent = ENT ? a.g_ent[r] : 0.0f, ent = ENT ? a.ent_in[r] : 0.0f;
+    const quasar_logprob_stat st = a.stats_in[r];
+    const T* row = (const T*)a.logits + r * a.ld;
+    T* out = (T*)a.grad + r * a.grad_ld;
+    const Slice s = slice_of(row, a.V, part, parts);
+    Coef c = fill_coef(target >= a.V);
+    if (target >= 0 && target < a.V) {
+        const float R = st.max * k;
+        const bool wide = fabsf(R) > WIDE && !isinf(st.max);
+        // st.sum stands against M * k, the loop's terms against R
+        const float S = wide || isinf(st.max) ? st.sum : st.sum * ex2_approx(fmaf(st.max, k, -R));
+        c = make_coef(st.max, R, wide, S, ENT ? ent - logf(S) : 0.0f, g_lp, g_ent, (float)a.inv_t);
+    }
+    const int hot = target >= s.head ? (target - s.head) / N - s.lo : -1;
+    const bool mine = elementwise(c) && hot >= 0 && hot < s.n && hot % NT == (int)threadIdx.x;
+    const float lt = mine ? widen1(row[target]) : 0.0f;  // read before its pack is written over
+    if (s.edge >= 0) put_edge<T, ENT>(out, s.edge, target, elementwise(c) ? widen1(row[s.edge]) : 0.0f, c, k);
+    const uint4* src = reinterpret_cast<const uint4*>(row + s.head) + s.lo + threadIdx.x;
+    T* dst = out + s.head + (int64_t)(s.lo + (int)threadIdx.x) * N;
+    if (((uintptr_t)dst & 15) == 0 && c.kind == ROW_SUM) {
+        uint4* d = reinterpret_cast<uint4*>(dst);
+        const int n = s.n - (int)threadIdx.x;
+        int v = 0;
+        for (; v + (U - 1) * NT < n; v += NT * U) {
+            uint4 p[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) p[u] = load_pack(src + v + u * NT);
+#pragma unroll
+            for (int u = 0; u < U; u++) d[v + u * NT] = grad_of<T, ENT>(p[u], c, k);
+        }
         uint4 p[U];
 #pragma unroll
         for (int u = 0; u < U; u++)
-            if (v0 + u * NT < hi && c.kind == 0) p[u] = load_pack(src + v0 + u * NT);
+            if (v + u * NT < n) p[u] = load_pack(src + v + u * NT);
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int v = v0 + u * NT;
-            if (v >= hi) continue;
-            float x[N];
-            if (c.kind == 0) {
-                widen(p[u], x, (T*)nullptr);
-#pragma unroll
-                for (int i = 0; i < N; i++) x[i] = grad1<ENT>(c, x[i], k);
-                if (v == hot) {
-                    const int j = (target - sp.head) % N;
-#pragma unroll
-                    for (int i = 0; i < N; i++)
-                        if (i == j) x[i] += c.one;
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < N; i++) x[i] = fill;
-            }
-            if (same)
-                reinterpret_cast<uint4*>(dst)[v] = narrow(x, (T*)nullptr);
-            else
-#pragma unroll
-                for (int i = 0; i < N; i++) put1(dst + (int64_t)v * N + i, x[i]);
-        }
-    }
-}
-
-// ---- kernels -----------------------------------------------------------------
-
-// One cluster per row: log-probability, entropy, and with POLICY the policy
-// loss and the gradient.
-template <typename T, bool ENT, bool POLICY>
-__global__ void __launch_bounds__(NT) rows_kernel(const Args a) {
-    __shared__ Part parts[MAXC * NW];
-    const int C = (int)cluster_size(), rank = (int)cluster_rank();
-    const int r = (int)(blockIdx.x / C);
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const T* row = (const T*)a.logits + (int64_t)r * a.ld;
-    const int target = a.targets[r];
-    const float k = a.k;
-    if (C > 1) cluster_arrive();  // the peers' shared memory is written below
-
-    double weight = 1.0;
-    if (POLICY) weight = a.weight ? (double)a.weight[r] : 1.0 / a.rows;
-    const bool live = target >= 0 && weight != 0.0;
-    const bool bad = target >= a.V;
-    Coef c;
-    c.m = c.a = c.b = c.one = 0.0f;
-    c.kind = 1;
-    float lt = 0.0f;
-    Acc acc{NEG, -INFINITY, 0.0f, 0.0f};
-    if (live && !bad) {
-        constexpr int N = Type<T>::N;
-        lt = widen1(row[target]);
-        const Span sp = span_of(row, a.V);
-        if (rank == 0 && tid < sp.head + sp.tail) {
-            const float x[2] = {widen1(row[tid < sp.head ? tid : a.V - sp.tail + (tid - sp.head)]), -INFINITY};
-            add<ENT>(acc, x, k);
-        }
-        const int lo = (int)((int64_t)sp.packs * rank / C), hi = (int)((int64_t)sp.packs * (rank + 1) / C);
-        const uint4* src = reinterpret_cast<const uint4*>(row + sp.head);
-        for (int v0 = lo + tid; v0 < hi; v0 += NT * U) {
-            uint4 p[U];
-#pragma unroll
-            for (int u = 0; u < U; u++) {
-                p[u] = make_uint4(Type<T>::NEG_INF, Type<T>::NEG_INF, Type<T>::NEG_INF, Type<T>::NEG_INF);
-                if (v0 + u * NT < hi) p[u] = load_pack(src + v0 + u * NT);
-            }
-#pragma unroll
-            for (int u = 0; u < U; u++) {
-                float x[N];
-                widen(p[u], x, (T*)nullptr);
-                add<ENT>(acc, x, k);
-            }
-        }
-    }
-    const Part mine = warp_part(acc, k);
-    if (C > 1) {
-        cluster_wait();
-        if (lane < C) remote_store(&parts[rank * NW + warp], lane, mine);
-        cluster_arrive();
-        cluster_wait();
+        for (int u = 0; u < U; u++)
+            if (v + u * NT < n) d[v + u * NT] = grad_of<T, ENT>(p[u], c, k);
     } else {
-        if (lane == 0) parts[warp] = mine;
-        __syncthreads();
+        grad_plain<T, ENT>(row, out, s.head, s.lo, s.lo + s.n, c, k, NT);
     }
-    // every warp joins the C * NW parts in the same order
-    float M = -INFINITY;
-    double S = 0.0, Q = 0.0;
-    for (int i = lane; i < C * NW; i += 32) M = fmaxf(M, parts[i].m);
-    M = warp_max(M);
-    for (int i = lane; i < C * NW; i += 32) {
-        Part p = parts[i];
-        rebase(p.s, p.q, p.m, M, k);
-        S += p.s, Q += p.q;
-    }
-    S = warp_sum(S), Q = warp_sum(Q);
-
-    double lp = 0.0, H = 0.0, loss = 0.0;
-    if (live) {
-        const bool none = M == -INFINITY && S == 0.0;
-        const double lnS = log(S);
-        lp = none ? -INFINITY : (double)(lt - M) * ((double)k * LN2) - lnS;
-        if (ENT) H = none ? 0.0 : lnS - LN2 * (Q / S);
-        if (bad) lp = H = NAN;
-        if (POLICY) {
-            const double adv = a.adv[r], ratio = exp(lp - (double)a.old_lp[r]);
-            const double lo = 1.0 - a.clip_lo, hi = 1.0 + a.clip_hi;
-            const double fit = ratio < lo ? lo : ratio > hi ? hi : ratio;  // NaN stays
-            const double x = ratio * adv, y = fit * adv;
-            loss = x <= y ? -x : y < x ? -y : NAN;
-            double g = x <= y ? -x : y < x ? 0.0 : NAN;
-            if (a.kl != 0.0) {
-                const double u = (double)a.ref_lp[r] - lp, eu = exp(u);
-                loss += a.kl * (eu - u - 1.0);
-                g += a.kl * (1.0 - eu);
-            }
-            if (ENT && a.ec != 0.0) loss -= a.ec * H;
-            if (a.grad) {
-                c = make_coef(M, S, H, g * weight * a.scale, ENT ? -a.ec * weight * a.scale : 0.0, a.inv_t);
-                if (bad) c.kind = 2;
-            }
-        }
-    }
-    if (rank == 0 && tid == 0) {
-        a.logprob[r] = (float)lp;
-        if (a.entropy) a.entropy[r] = (float)H;
-        if (a.stats) a.stats[r] = {live && !bad ? M : 0.0f, live && !bad ? (float)S : 0.0f};
-        if (a.row_grad) a.row_grad[r] = 0.0f;
-        if (POLICY) a.row_loss[r] = (float)loss;
-    }
-    if (POLICY && a.grad) grad_slice<T, ENT>(row, (T*)a.grad + (int64_t)r * a.grad_ld, a.V, target, c, k, rank, C);
+    if (mine) put1(out + target, grad1<ENT>(c, lt, k) + c.one);
 }
 
-// The gradient from given statistics and per-row derivatives; gridDim.y CTAs
-// per row.
-template <typename T, bool ENT>
-__global__ void __launch_bounds__(NT) grad_kernel(const Args a) {
-    const int r = (int)blockIdx.x;
-    const int target = a.targets[r];
-    Coef c;
-    c.m = c.a = c.b = c.one = 0.0f;
-    c.kind = 1;
-    if (target >= a.V) {
-        c.kind = 2;
-    } else if (target >= 0) {
-        const quasar_logprob_stat s = a.stats_in[r];
-        c = make_coef(s.max, s.sum, ENT ? a.ent_in[r] : 0.0, a.g_lp[r], ENT ? a.g_ent[r] : 0.0, a.inv_t);
-    }
-    grad_slice<T, ENT>((const T*)a.logits + (int64_t)r * a.ld, (T*)a.grad + (int64_t)r * a.grad_ld, a.V, target, c, a.k,
-                       (int)blockIdx.y, (int)gridDim.y);
-}
+// ---- pairs and sums --------------------------------------------------------------
 
-// Sum over 128 threads, the same in every run; all threads get it.
+// Sum over a CTA, the same in every run; all threads get it.
 __device__ __forceinline__ double cta_sum(double x, double* buf, int threads) {
     x = warp_sum(x);
     __syncthreads();
@@ -418,6 +1122,8 @@ __device__ __forceinline__ double cta_sum(double x, double* buf, int threads) {
 // One CTA per pair.
 __global__ void __launch_bounds__(128) pair_kernel(const PairArgs p) {
     __shared__ double buf[4];
+    wait_before();
+    launch_next();
     const int i = blockIdx.x, tid = threadIdx.x;
     const int at[3] = {p.cu[2 * i], p.cu[2 * i + 1], p.cu[2 * i + 2]};
     const bool ok = at[0] >= 0 && at[0] <= at[1] && at[1] <= at[2] && at[2] <= p.rows;
@@ -457,47 +1163,159 @@ __global__ void __launch_bounds__(128) pair_kernel(const PairArgs p) {
                 if (p.targets[r] >= 0) p.row_grad[r] = (float)((s ? -g : g) * by[s]);
 }
 
-__global__ void __launch_bounds__(1024) weighted_sum_kernel(const float* x, const float* w, int n, float* out) {
-    __shared__ double buf[32];
+// One CTA: the same order of sums in every run.
+__global__ void __launch_bounds__(512) weighted_sum_kernel(const float* x, const float* w, int n, float* out) {
+    __shared__ double buf[16];
+    wait_before();
+    launch_next();
     double s = 0.0;
-    for (int i = threadIdx.x; i < n; i += 1024) {
+    for (int i = threadIdx.x; i < n; i += 512) {
         const double wi = w ? (double)w[i] : 1.0;
         if (wi != 0.0) s += wi * (double)x[i];
     }
-    s = cta_sum(s, buf, 1024);
+    s = cta_sum(s, buf, 512);
     if (threadIdx.x == 0) out[0] = (float)(w || n == 0 ? s : s / n);
 }
 
+
 // ---- launchers ---------------------------------------------------------------
 
-// CTAs per row.
-static int row_cluster(const Args& a) {
-    int C = MAXC;
-    while (C > 1 && (int64_t)a.rows * C > INT32_MAX) C /= 2;  // the grid's limit
+// Starts `kern` behind what is on the stream; with `early` before that has
+// ended (the kernel waits for it itself), which hides the launch.
+template <typename... P, typename... X>
+static cudaError_t launch(void (*kern)(P...), unsigned grid, int block, size_t smem, int cluster, bool early, cudaStream_t st, X... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3((unsigned)block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[2];
+    unsigned n = 0;
+    if (cluster > 0) {
+        at[n].id = cudaLaunchAttributeClusterDimension;
+        at[n].val.clusterDim.x = (unsigned)cluster;
+        at[n].val.clusterDim.y = at[n].val.clusterDim.z = 1;
+        n++;
+    }
+    if (early) {
+        at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[n].val.programmaticStreamSerializationAllowed = 1;
+        n++;
+    }
+    cfg.attrs = at;
+    cfg.numAttrs = n;
+    return cudaLaunchKernelEx(&cfg, kern, args...);
+}
+
+static constexpr int SMS = 148;
+
+// CTAs per row: clusters of up to 8 while the rows alone leave SMs idle, and
+// the slices are not under 8 KB. At V = 151936, fp32: 1 row 6.2 us with 8
+// CTAs and 22 with one; 256 rows 28.7 us with 2, 31.1 with 1, 33.7 with 4.
+static int row_cluster(int64_t rows, int64_t row_bytes) {
+    int C = 1;
+    while (C < MAXC && rows * C < 2 * SMS && row_bytes >= (int64_t)C * 2 * 8192) C *= 2;
     return C;
 }
 
+template <typename T, bool ENT, bool POLICY, int NT>
+static cudaError_t rows_launch(const Args& a, int C, cudaStream_t st) {
+    return launch(rows_kernel<T, ENT, POLICY, NT>, (unsigned)a.rows * (unsigned)C, NT, 0, C, false, st, a);
+}
+
+// Short rows take small CTAs, of which an SM runs more at once: a CTA's start,
+// its barrier and its scalars take about 4 us whatever its slice. bf16 rows of
+// 38 KB, 16384 of them: 247 us with 128 threads, 274 with 256 (policy loss and
+// gradient); fp32 rows of 76 KB, 2000 of them: 63 us with 256, 70 with 128.
 template <typename T, bool ENT, bool POLICY>
-static cudaError_t rows_launch(const Args& a, cudaStream_t st) {
-    const int C = row_cluster(a);
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)a.rows * (unsigned)C);
-    cfg.blockDim = dim3(NT);
-    cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = C;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, rows_kernel<T, ENT, POLICY>, a);
+static cudaError_t rows_by_size(const Args& a, cudaStream_t st) {
+    const int64_t row_bytes = (int64_t)a.V * sizeof(T);
+    const int C = row_cluster(a.rows, row_bytes);
+    if (C == 1 && row_bytes <= 4096) return rows_launch<T, ENT, POLICY, 32>(a, C, st);
+    if (C == 1 && row_bytes <= 49152) return rows_launch<T, ENT, POLICY, 128>(a, C, st);
+    return rows_launch<T, ENT, POLICY, 256>(a, C, st);
+}
+
+// Long rows: one CTA of 512 consumers per SM with chunks of 32 KB. Middle
+// ones, of which an SM can hold two, two CTAs of 256 with chunks of 20 KB.
+using StreamLong = StreamShape<512, 1, 4, 6>;
+using StreamMiddle = StreamShape<256, 2, 5, 5>;
+static constexpr int64_t STREAM_MIN = 96 * 1024, STREAM_MIDDLE = 128 * 1024, STREAM_L2 = 32 << 20;
+
+static std::mutex g_mu;
+
+template <typename T, bool ENT, typename Shape>
+static cudaError_t stream_launch(const Args& a, int C, cudaStream_t st) {
+    auto kern = stream_kernel<T, ENT, Shape>;
+    const size_t smem = (size_t)Shape::STAGES * Shape::CH;
+    // per device: whether the kernel is set up, and the clusters that fit
+    static int most[64][MAXC + 1];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    int clusters;
+    {
+        std::lock_guard<std::mutex> lock(g_mu);
+        clusters = most[dev][C];
+        if (!clusters) {
+            e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+            if (e != cudaSuccess) return e;
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3((unsigned)C);
+            cfg.blockDim = dim3(Shape::NT + 64);
+            cfg.dynamicSmemBytes = smem;
+            cudaLaunchAttribute at[1];
+            at[0].id = cudaLaunchAttributeClusterDimension;
+            at[0].val.clusterDim.x = (unsigned)C;
+            at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+            cfg.attrs = at;
+            cfg.numAttrs = 1;
+            e = cudaOccupancyMaxActiveClusters(&clusters, kern, &cfg);
+            if (e != cudaSuccess) return e;
+            if (clusters < 1) return cudaErrorInvalidConfiguration;
+            most[dev][C] = clusters;
+        }
+    }
+    for (int64_t r0 = 0; r0 < a.rows; r0 += STREAM_ROWS) {
+        Args b = a;
+        b.rows = (int)(a.rows - r0 < STREAM_ROWS ? a.rows - r0 : STREAM_ROWS);
+        b.logits = (const T*)a.logits + r0 * a.ld;
+        b.grad = (T*)a.grad + r0 * a.grad_ld;
+        b.targets += r0, b.logprob += r0, b.row_loss += r0, b.old_lp += r0, b.adv += r0;
+        if (b.entropy) b.entropy += r0;
+        if (b.ref_lp) b.ref_lp += r0;
+        if (b.weight) b.weight += r0;
+        const int n = b.rows < clusters ? b.rows : clusters;
+        e = launch(kern, (unsigned)(n * C), Shape::NT + 64, smem, C, false, st, b);
+        if (e != cudaSuccess) return e;
+    }
+    return cudaSuccess;
+}
+
+// The policy loss with its gradient: the streaming kernel where a row is long
+// enough for its chunks and there are rows for several turns of every cluster
+// (policy loss and gradient at V = 151936: fp32, 4096 rows 803 us streamed,
+// 899 with a cluster of 8 per row; bf16, 600 rows 82 and 88 us, 148 rows 27
+// and 29; 50021 f16 columns, 1000 rows 47 and 52 us, 300 rows 25 and 22).
+template <typename T, bool ENT>
+static cudaError_t policy_by_size(const Args& a, cudaStream_t st) {
+    const int64_t row_bytes = (int64_t)a.V * sizeof(T);
+    if (row_bytes >= STREAM_MIN && row_bytes <= STREAM_MIDDLE && a.rows >= 4 * SMS) return stream_launch<T, ENT, StreamMiddle>(a, 1, st);
+    if (row_bytes > STREAM_MIDDLE && a.rows >= SMS) {
+        int C = 1;
+        while (C < MAXC && SMS / C * row_bytes > STREAM_L2) C *= 2;
+        return stream_launch<T, ENT, StreamLong>(a, C, st);
+    }
+    return rows_by_size<T, ENT, true>(a, st);
 }
 
 template <typename T>
 static cudaError_t rows_typed(const Args& a, cudaStream_t st) {
     const bool ent = a.entropy != nullptr || a.ec != 0.0;
-    if (a.adv) return ent ? rows_launch<T, true, true>(a, st) : rows_launch<T, false, true>(a, st);
-    return ent ? rows_launch<T, true, false>(a, st) : rows_launch<T, false, false>(a, st);
+    if (!a.adv) return ent ? rows_by_size<T, true, false>(a, st) : rows_by_size<T, false, false>(a, st);
+    if (!a.grad) return ent ? rows_by_size<T, true, true>(a, st) : rows_by_size<T, false, true>(a, st);
+    return ent ? policy_by_size<T, true>(a, st) : policy_by_size<T, false>(a, st);
 }
 
 cudaError_t launch_rows(const Args& a, int dtype, cudaStream_t st) {
@@ -506,14 +1324,16 @@ cudaError_t launch_rows(const Args& a, int dtype, cudaStream_t st) {
     return rows_typed<__nv_bfloat16>(a, st);
 }
 
+// Slices of about 76 KB, smaller ones where the rows are few.
 template <typename T>
 static cudaError_t grad_typed(const Args& a, cudaStream_t st) {
-    const dim3 grid((unsigned)a.rows, 8);
-    if (a.g_ent)
-        grad_kernel<T, true><<<grid, NT, 0, st>>>(a);
-    else
-        grad_kernel<T, false><<<grid, NT, 0, st>>>(a);
-    return cudaPeekAtLastError();
+    const int64_t row_bytes = (int64_t)a.V * sizeof(T);
+    int64_t parts = (row_bytes + 77823) / 77824;
+    while (parts * a.rows < 4 * SMS && row_bytes > parts * 2 * 8192) parts *= 2;
+    if (parts * a.rows > INT32_MAX) parts = 1;
+    const unsigned grid = (unsigned)(a.rows * parts);
+    if (a.g_ent) return launch(grad_kernel<T, true>, grid, 256, 0, 0, true, st, a, (int)parts);
+    return launch(grad_kernel<T, false>, grid, 256, 0, 0, true, st, a, (int)parts);
 }
 
 cudaError_t launch_grad(const Args& a, int dtype, cudaStream_t st) {
@@ -522,14 +1342,10 @@ cudaError_t launch_grad(const Args& a, int dtype, cudaStream_t st) {
     return grad_typed<__nv_bfloat16>(a, st);
 }
 
-cudaError_t launch_pairs(const PairArgs& p, cudaStream_t st) {
-    pair_kernel<<<p.pairs, 128, 0, st>>>(p);
-    return cudaPeekAtLastError();
-}
+cudaError_t launch_pairs(const PairArgs& p, cudaStream_t st) { return launch(pair_kernel, (unsigned)p.pairs, 128, 0, 0, true, st, p); }
 
 cudaError_t launch_weighted_sum(const float* x, const float* w, int n, float* out, cudaStream_t st) {
-    weighted_sum_kernel<<<1, 1024, 0, st>>>(x, w, n, out);
-    return cudaPeekAtLastError();
+    return launch(weighted_sum_kernel, 1u, 512, 0, 0, true, st, x, w, n, out);
 }
 
 }  // namespace loss

@@ -27,6 +27,7 @@ struct Args {
     const float* adv;
     const float* ref_lp;
     const float* weight;
+    double mean;  // the weight of a row with weight == NULL
     double clip_lo, clip_hi, kl, ec;
     float* row_loss;
     double scale;  // gradient scale
