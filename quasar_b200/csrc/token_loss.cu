@@ -1236,9 +1236,9 @@ static cudaError_t rows_by_size(const Args& a, cudaStream_t st) {
     return rows_launch<T, ENT, POLICY, 256>(a, C, st);
 }
 
-// Long rows: one CTA of 512 consumers per SM with chunks of 32 KB. Middle
+// Long rows: one CTA of 640 consumers per SM with chunks of 30 KB. Middle
 // ones, of which an SM can hold two, two CTAs of 256 with chunks of 20 KB.
-using StreamLong = StreamShape<512, 1, 4, 6>;
+using StreamLong = StreamShape<640, 1, 3, 7>;
 using StreamMiddle = StreamShape<256, 2, 5, 5>;
 static constexpr int64_t STREAM_MIN = 96 * 1024, STREAM_MIDDLE = 128 * 1024, STREAM_L2 = 32 << 20;
 

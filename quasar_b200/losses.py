@@ -18,6 +18,7 @@ from typing import NamedTuple, Optional
 from ._lib import BF16, F16, F32, check, lib
 
 _DTYPES = {}  # torch dtype -> the C constant; filled at the first call, torch being imported only then
+_raw = None   # the current stream's handle by device index, where torch has a way to it without a Stream object (2 us)
 
 
 class PolicyParams(ctypes.Structure):
@@ -56,47 +57,56 @@ class PreferenceLoss(NamedTuple):
     grad: Optional[torch.Tensor]      # [rows, V] of the logits' type, or None
 
 
-def _rows(logits, targets):
-    """Checks logits and targets; returns (rows, V, the C dtype)."""
+def _torch():
+    """torch, imported at the first call; fills the table of types."""
     import torch
     if not _DTYPES:
+        global _raw
+        _raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
         _DTYPES.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
-    if logits.dim() != 2 or logits.dtype not in _DTYPES:
+    return torch
+
+
+def _rows(logits, targets):
+    """Checks logits and targets; returns (torch, rows, V, the C dtype, the row stride, the device)."""
+    torch = _torch()
+    dt = _DTYPES.get(logits.dtype)
+    if logits.dim() != 2 or dt is None:
         raise ValueError("logits must be a [rows, V] float32, float16 or bfloat16 tensor")
     if not logits.is_cuda:
         raise ValueError("logits must be a CUDA tensor")
     rows, V = logits.shape
-    if logits.stride(1) != 1 and V > 1:
+    ld, unit = logits.stride()
+    if unit != 1 and V > 1:
         raise ValueError("logits must have unit column stride")
-    if rows > 1 and logits.stride(0) < V:
+    if rows < 2:
+        ld = max(V, 1)  # a tensor of one row or none may have any row stride
+    elif ld < V:
         raise ValueError("rows of logits must not overlap")
-    _vec(targets, "targets", (rows,), torch.int32, logits)
-    return rows, V, _DTYPES[logits.dtype]
+    device = logits.device
+    _vec(targets, "targets", (rows,), torch.int32, device)
+    return torch, rows, V, dt, ld, device
 
 
-def _vec(t, name, shape, dtype, logits):
-    if t.shape != shape or t.dtype != dtype or t.device != logits.device or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {list(shape)} on {logits.device}, got "
+def _vec(t, name, shape, dtype, device):
+    if t.dtype is not dtype or t.shape != shape or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {list(shape)} on {device}, got "
                          f"{t.dtype} {list(t.shape)} on {t.device}")
 
 
 def _ld(t):
-    """Row stride in elements (a tensor of one row or none may have any)."""
     return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
 
 
-def _like(logits):
+def _like(torch, logits, rows, V, ld):
     """A gradient buffer of the logits' shape whose rows have the 16-byte phase of the logits' rows."""
-    import torch
-    rows, V = logits.shape
-    ld, size = _ld(logits), logits.element_size()
-    if ld == V and logits.data_ptr() % 16 == 0:
-        return torch.empty((rows, V), dtype=logits.dtype, device=logits.device)
-    per = 16 // size
-    first = logits.data_ptr() % 16 // size
+    phase = logits.data_ptr() & 15
+    if ld == V and phase == 0:
+        return logits.new_empty((rows, V))
+    size = logits.element_size()
+    per, first = 16 // size, phase // size
     ld = V + (ld - V) % per  # the shortest stride with the same phases
-    flat = torch.empty(first + rows * ld, dtype=logits.dtype, device=logits.device)
-    return flat.as_strided((rows, V), (ld, 1), first)
+    return logits.new_empty(first + rows * ld).as_strided((rows, V), (ld, 1), first)
 
 
 def _check_grad(grad, logits):
@@ -106,46 +116,36 @@ def _check_grad(grad, logits):
         raise ValueError("the gradient must have unit column stride and rows that do not overlap")
 
 
+def _grad_arg(torch, grad, logits):
+    """Checks the grad argument; returns the buffer that was passed, or None."""
+    if grad is True or grad is False:
+        return None
+    if not isinstance(grad, torch.Tensor):
+        raise ValueError("grad must be True (allocate), False (none) or a tensor to write")
+    _check_grad(grad, logits)
+    return grad
+
+
 def _p(t):
     return None if t is None else t.data_ptr()
 
 
-class _On:
-    """Makes the logits' device and the stream of the call current, and keeps the call's tensors from being
-    handed out again before that stream is done with them."""
-
-    def __init__(self, logits, stream, tensors):
-        self.device = logits.device.index
-        self.stream = stream
-        self.tensors = tensors
-
-    def __enter__(self):
-        import torch
-        self.before = None
-        if torch.cuda.current_device() != self.device:
-            self.before = torch.cuda.current_device()
-            torch.cuda.set_device(self.device)
-        current = torch.cuda.current_stream(self.device)
-        self.back = None
-        if self.stream is not None and self.stream != current:
-            if self.stream.device.index != self.device:
-                self.__exit__()
-                raise ValueError(f"the stream is on {self.stream.device}, the logits on cuda:{self.device}")
-            for t in self.tensors:
-                if t is not None:
-                    t.record_stream(self.stream)
-            self.back = current
-            torch.cuda.set_stream(self.stream)
-            current = self.stream
-        return current.cuda_stream
-
-    def __exit__(self, *exc):
-        import torch
-        if getattr(self, "back", None) is not None:
-            torch.cuda.set_stream(self.back)
-        if self.before is not None:
-            torch.cuda.set_device(self.before)
-        return False
+def _on(torch, device, stream, tensors, call):
+    """call(the C stream) with the logits' device and the stream of the call current, so that what it allocates
+    belongs to that stream; keeps the call's tensors from being handed out again before the stream is done."""
+    if stream is None and torch.cuda.current_device() == device.index:
+        return call(_raw(device.index) if _raw else torch.cuda.current_stream(device).cuda_stream)
+    with torch.cuda.device(device):
+        current = torch.cuda.current_stream(device)
+        if stream is None or stream == current:
+            return call(current.cuda_stream)
+        if stream.device != device:
+            raise ValueError(f"the stream is on {stream.device}, the logits on {device}")
+        for t in tensors:
+            if t is not None:
+                t.record_stream(stream)
+        with torch.cuda.stream(stream):
+            return call(stream.cuda_stream)
 
 
 def token_logprobs(logits, targets, *, temperature: float = 1.0, entropy: bool = False,
@@ -156,25 +156,26 @@ def token_logprobs(logits, targets, *, temperature: float = 1.0, entropy: bool =
     out: a TokenLogprobs of an earlier call whose tensors are written again (its entropy as ``entropy`` asks).
     Launches on ``stream`` (a torch.cuda.Stream; default: the current stream).
     """
-    import torch
-    rows, V, dt = _rows(logits, targets)
+    torch, rows, V, dt, ld, device = _rows(logits, targets)
+    f32 = torch.float32
     if out is not None:
-        _vec(out.logprob, "out.logprob", (rows,), torch.float32, logits)
-        _vec(out.stats, "out.stats", (rows, 2), torch.float32, logits)
+        _vec(out.logprob, "out.logprob", (rows,), f32, device)
+        _vec(out.stats, "out.stats", (rows, 2), f32, device)
         if entropy != (out.entropy is not None):
             raise ValueError("out.entropy must be a tensor if entropy is asked for, and None if not")
         if entropy:
-            _vec(out.entropy, "out.entropy", (rows,), torch.float32, logits)
-    with _On(logits, stream, (logits, targets, *(out or ()))) as st:
-        if out is None:
-            dev = logits.device
-            out = TokenLogprobs(torch.empty(rows, device=dev, dtype=torch.float32),
-                                torch.empty(rows, device=dev, dtype=torch.float32) if entropy else None,
-                                torch.empty((rows, 2), device=dev, dtype=torch.float32))
-        check(lib().quasar_token_logprobs(_p(logits), dt, _ld(logits), rows, V, _p(targets), temperature,
-                                          _p(out.logprob), _p(out.entropy), _p(out.stats), st),
+            _vec(out.entropy, "out.entropy", (rows,), f32, device)
+
+    def call(st):
+        o = out
+        if o is None:
+            e = logits.new_empty
+            o = TokenLogprobs(e(rows, dtype=f32), e(rows, dtype=f32) if entropy else None, e((rows, 2), dtype=f32))
+        check(lib().quasar_token_logprobs(logits.data_ptr(), dt, ld, rows, V, targets.data_ptr(), temperature,
+                                          o.logprob.data_ptr(), _p(o.entropy), o.stats.data_ptr(), st),
               "quasar_token_logprobs")
-    return out
+        return o
+    return _on(torch, device, stream, (logits, targets, *(out or ())), call)
 
 
 def token_logprobs_grad(logits, targets, stats, grad_logprob, *, entropy=None, grad_entropy=None,
@@ -185,32 +186,25 @@ def token_logprobs_grad(logits, targets, stats, grad_logprob, *, entropy=None, g
     temperature. out: a tensor of the logits' shape and type to write, which may be ``logits`` itself.
     Returns the gradient, of the logits' type.
     """
-    import torch
-    rows, V, dt = _rows(logits, targets)
-    _vec(stats, "stats", (rows, 2), torch.float32, logits)
-    _vec(grad_logprob, "grad_logprob", (rows,), torch.float32, logits)
+    torch, rows, V, dt, ld, device = _rows(logits, targets)
+    f32 = torch.float32
+    _vec(stats, "stats", (rows, 2), f32, device)
+    _vec(grad_logprob, "grad_logprob", (rows,), f32, device)
     if (entropy is None) != (grad_entropy is None):
         raise ValueError("pass entropy and grad_entropy together")
     if entropy is not None:
-        _vec(entropy, "entropy", (rows,), torch.float32, logits)
-        _vec(grad_entropy, "grad_entropy", (rows,), torch.float32, logits)
+        _vec(entropy, "entropy", (rows,), f32, device)
+        _vec(grad_entropy, "grad_entropy", (rows,), f32, device)
     if out is not None:
         _check_grad(out, logits)
-    with _On(logits, stream, (logits, targets, stats, grad_logprob, entropy, grad_entropy, out)) as st:
-        if out is None:
-            out = _like(logits)
-        check(lib().quasar_token_logprobs_grad(_p(logits), dt, _ld(logits), rows, V, _p(targets), temperature,
-                                               _p(stats), _p(entropy), _p(grad_logprob), _p(grad_entropy), _p(out),
-                                               _ld(out), st), "quasar_token_logprobs_grad")
-    return out
 
-
-def _grad_arg(grad, logits):
-    import torch
-    if isinstance(grad, torch.Tensor):
-        _check_grad(grad, logits)
-    elif grad is not True and grad is not False:
-        raise ValueError("grad must be True (allocate), False (none) or a tensor to write")
+    def call(st):
+        g = _like(torch, logits, rows, V, ld) if out is None else out
+        check(lib().quasar_token_logprobs_grad(logits.data_ptr(), dt, ld, rows, V, targets.data_ptr(), temperature,
+                                               stats.data_ptr(), _p(entropy), grad_logprob.data_ptr(), _p(grad_entropy),
+                                               g.data_ptr(), _ld(g), st), "quasar_token_logprobs_grad")
+        return g
+    return _on(torch, device, stream, (logits, targets, stats, grad_logprob, entropy, grad_entropy, out), call)
 
 
 def policy_loss(logits, targets, old_logprob, advantage, *, ref_logprob=None, weight=None, temperature: float = 1.0,
@@ -229,42 +223,42 @@ def policy_loss(logits, targets, old_logprob, advantage, *, ref_logprob=None, we
     none. grad_scale multiplies the gradient, not the loss. out: a PolicyLoss of an earlier call whose tensors
     other than grad are written again.
     """
-    import torch
-    rows, V, dt = _rows(logits, targets)
+    torch, rows, V, dt, ld, device = _rows(logits, targets)
     f32 = torch.float32
-    _vec(old_logprob, "old_logprob", (rows,), f32, logits)
-    _vec(advantage, "advantage", (rows,), f32, logits)
+    shape = (rows,)
+    _vec(old_logprob, "old_logprob", shape, f32, device)
+    _vec(advantage, "advantage", shape, f32, device)
     if ref_logprob is not None:
-        _vec(ref_logprob, "ref_logprob", (rows,), f32, logits)
+        _vec(ref_logprob, "ref_logprob", shape, f32, device)
     elif kl_coef != 0.0:
         raise ValueError("kl_coef needs ref_logprob")
     if weight is not None:
-        _vec(weight, "weight", (rows,), f32, logits)
+        _vec(weight, "weight", shape, f32, device)
     want = entropy or entropy_coef != 0.0
-    _grad_arg(grad, logits)
+    buf = _grad_arg(torch, grad, logits)
     if out is not None:
-        _vec(out.loss, "out.loss", (), f32, logits)
-        _vec(out.logprob, "out.logprob", (rows,), f32, logits)
-        _vec(out.row_loss, "out.row_loss", (rows,), f32, logits)
+        _vec(out.loss, "out.loss", (), f32, device)
+        _vec(out.logprob, "out.logprob", shape, f32, device)
+        _vec(out.row_loss, "out.row_loss", shape, f32, device)
         if want != (out.entropy is not None):
             raise ValueError("out.entropy must be a tensor if the entropy is computed, and None if not")
         if want:
-            _vec(out.entropy, "out.entropy", (rows,), f32, logits)
+            _vec(out.entropy, "out.entropy", shape, f32, device)
     prm = PolicyParams(temperature, clip_low, clip_high, kl_coef, entropy_coef, grad_scale)
-    buf = grad if isinstance(grad, torch.Tensor) else None
-    with _On(logits, stream, (logits, targets, old_logprob, advantage, ref_logprob, weight, buf, *(out or ()))) as st:
-        dev = logits.device
+
+    def call(st):
+        g = _like(torch, logits, rows, V, ld) if grad is True else buf
         if out is None:
-            out = PolicyLoss(torch.empty((), device=dev, dtype=f32), torch.empty(rows, device=dev, dtype=f32),
-                             torch.empty(rows, device=dev, dtype=f32) if want else None,
-                             torch.empty(rows, device=dev, dtype=f32), None)
-        if grad is True:
-            buf = _like(logits)
-        check(lib().quasar_policy_loss(_p(logits), dt, _ld(logits), rows, V, _p(targets), _p(old_logprob),
-                                       _p(advantage), _p(ref_logprob), _p(weight), ctypes.addressof(prm),
-                                       _p(out.logprob), _p(out.entropy), _p(out.row_loss), _p(out.loss), _p(buf),
-                                       0 if buf is None else _ld(buf), st), "quasar_policy_loss")
-    return out._replace(grad=buf)
+            e = logits.new_empty
+            o = PolicyLoss(e((), dtype=f32), e(rows, dtype=f32), e(rows, dtype=f32) if want else None, e(rows, dtype=f32), g)
+        else:
+            o = PolicyLoss(out.loss, out.logprob, out.entropy, out.row_loss, g)
+        check(lib().quasar_policy_loss(logits.data_ptr(), dt, ld, rows, V, targets.data_ptr(), old_logprob.data_ptr(),
+                                       advantage.data_ptr(), _p(ref_logprob), _p(weight), ctypes.addressof(prm), o.logprob.data_ptr(),
+                                       _p(o.entropy), o.row_loss.data_ptr(), o.loss.data_ptr(), _p(g),
+                                       0 if g is None else _ld(g), st), "quasar_policy_loss")
+        return o
+    return _on(torch, device, stream, (logits, targets, old_logprob, advantage, ref_logprob, weight, buf, *(out or ())), call)
 
 
 def preference_loss(logits, targets, cu_seqlens, *, ref_logprob=None, pair_weight=None, temperature: float = 1.0,
@@ -280,37 +274,38 @@ def preference_loss(logits, targets, cu_seqlens, *, ref_logprob=None, pair_weigh
       loss      = sum(pair_weight * pair_loss)                  (pair_weight None: 1/pairs each)
     grad, grad_scale, out: as for ``policy_loss``.
     """
-    import torch
-    rows, V, dt = _rows(logits, targets)
+    torch, rows, V, dt, ld, device = _rows(logits, targets)
     f32 = torch.float32
     if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] % 2 == 0:
         raise ValueError("cu_seqlens must have 2 * pairs + 1 offsets")
     n = cu_seqlens.shape[0] - 1
-    _vec(cu_seqlens, "cu_seqlens", (n + 1,), torch.int32, logits)
+    _vec(cu_seqlens, "cu_seqlens", (n + 1,), torch.int32, device)
     if ref_logprob is not None:
-        _vec(ref_logprob, "ref_logprob", (n,), f32, logits)
+        _vec(ref_logprob, "ref_logprob", (n,), f32, device)
     if pair_weight is not None:
-        _vec(pair_weight, "pair_weight", (n // 2,), f32, logits)
-    _grad_arg(grad, logits)
+        _vec(pair_weight, "pair_weight", (n // 2,), f32, device)
+    buf = _grad_arg(torch, grad, logits)
     if out is not None:
         for name, shape in (("loss", ()), ("pair_loss", (n // 2,)), ("seq_logprob", (n,)), ("logprob", (rows,)),
                             ("stats", (rows, 2)), ("row_grad", (rows,))):
-            _vec(getattr(out, name), "out." + name, shape, f32, logits)
+            _vec(getattr(out, name), "out." + name, shape, f32, device)
     prm = PreferenceParams(temperature, beta, label_smoothing, grad_scale, 1 if length_normalize else 0, 0)
-    buf = grad if isinstance(grad, torch.Tensor) else None
-    with _On(logits, stream, (logits, targets, cu_seqlens, ref_logprob, pair_weight, buf, *(out or ()))) as st:
-        dev = logits.device
+
+    def call(st):
+        g = _like(torch, logits, rows, V, ld) if grad is True else buf
         if out is None:
-            e = lambda *shape: torch.empty(shape, device=dev, dtype=f32)  # noqa: E731
-            out = PreferenceLoss(e(), e(n // 2), e(n), e(rows), e(rows, 2), e(rows), None)
-        if grad is True:
-            buf = _like(logits)
-        check(lib().quasar_preference_loss(_p(logits), dt, _ld(logits), rows, V, _p(targets), _p(cu_seqlens), n // 2,
-                                           _p(ref_logprob), _p(pair_weight), ctypes.addressof(prm), _p(out.logprob),
-                                           _p(out.seq_logprob), _p(out.pair_loss), _p(out.loss), _p(out.stats),
-                                           _p(out.row_grad), _p(buf), 0 if buf is None else _ld(buf), st),
+            e = logits.new_empty
+            o = PreferenceLoss(e((), dtype=f32), e(n // 2, dtype=f32), e(n, dtype=f32), e(rows, dtype=f32),
+                               e((rows, 2), dtype=f32), e(rows, dtype=f32), g)
+        else:
+            o = PreferenceLoss(*out[:6], g)
+        check(lib().quasar_preference_loss(logits.data_ptr(), dt, ld, rows, V, targets.data_ptr(), cu_seqlens.data_ptr(),
+                                           n // 2, _p(ref_logprob), _p(pair_weight), ctypes.addressof(prm), o.logprob.data_ptr(),
+                                           o.seq_logprob.data_ptr(), o.pair_loss.data_ptr(), o.loss.data_ptr(),
+                                           o.stats.data_ptr(), o.row_grad.data_ptr(), _p(g), 0 if g is None else _ld(g), st),
               "quasar_preference_loss")
-    return out._replace(grad=buf)
+        return o
+    return _on(torch, device, stream, (logits, targets, cu_seqlens, ref_logprob, pair_weight, buf, *(out or ())), call)
 
 
 __all__ = ["TokenLogprobs", "PolicyLoss", "PreferenceLoss", "PolicyParams", "PreferenceParams", "token_logprobs",
