@@ -367,7 +367,7 @@ __device__ __forceinline__ Coef finish_row(const Args& a, int64_t r, const Row& 
         float g = x <= y ? -x : y < x ? 0.0f : NAN;
         if (a.kl != 0.0) {
             const float u = (float)((double)in.ref_lp - lp), eu = expm1f(u);
-            loss += (float)a.kl * (eu - u);
+            loss += (float)a.kl * (isinf(eu) ? eu : eu - u);
             g -= (float)a.kl * eu;
         }
         if (ENT && a.ec != 0.0) loss -= (float)a.ec * H;
@@ -1131,7 +1131,7 @@ __global__ void __launch_bounds__(128) pair_kernel(const PairArgs p) {
     if (ok) {
         for (int s = 0; s < 2; s++) {
             double x = 0.0, c = 0.0;
-            for (int r = at[s] + tid; r < at[s + 1]; r += 128)
+            for (int64_t r = at[s] + tid; r < at[s + 1]; r += 128)
                 if (p.targets[r] >= 0) x += (double)p.logprob[r], c += 1.0;
             sum[s] = cta_sum(x, buf, 128);
             n[s] = cta_sum(c, buf, 128);
@@ -1149,7 +1149,8 @@ __global__ void __launch_bounds__(128) pair_kernel(const PairArgs p) {
     const double tail = log1p(exp(-fabs(x)));
     const double up = fmax(-x, 0.0) + tail, down = fmax(x, 0.0) + tail;
     const double sn = 1.0 / (1.0 + exp(x)), sp = 1.0 / (1.0 + exp(-x));
-    const double loss = (1.0 - p.eps) * up + (p.eps != 0.0 ? p.eps * down : 0.0);
+    // a share of 0 takes nothing, of an infinite loss either
+    const double loss = (p.eps != 1.0 ? (1.0 - p.eps) * up : 0.0) + (p.eps != 0.0 ? p.eps * down : 0.0);
     const double w = p.weight ? (double)p.weight[i] : 1.0 / p.pairs;
     const double g = -p.beta * ((1.0 - p.eps) * sn - p.eps * sp) * w * p.scale;
     if (tid == 0) {
@@ -1159,7 +1160,7 @@ __global__ void __launch_bounds__(128) pair_kernel(const PairArgs p) {
     }
     if (ok)
         for (int s = 0; s < 2; s++)
-            for (int r = at[s] + tid; r < at[s + 1]; r += 128)
+            for (int64_t r = at[s] + tid; r < at[s + 1]; r += 128)
                 if (p.targets[r] >= 0) p.row_grad[r] = (float)((s ? -g : g) * by[s]);
 }
 
@@ -1169,7 +1170,7 @@ __global__ void __launch_bounds__(512) weighted_sum_kernel(const float* x, const
     wait_before();
     launch_next();
     double s = 0.0;
-    for (int i = threadIdx.x; i < n; i += 512) {
+    for (int64_t i = threadIdx.x; i < n; i += 512) {
         const double wi = w ? (double)w[i] : 1.0;
         if (wi != 0.0) s += wi * (double)x[i];
     }

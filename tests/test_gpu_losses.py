@@ -12,6 +12,9 @@ sign; the target's own t adds 3 |t| 2^-24 and the output's rounding |lp| 2^-24.
 The bounds below are the worst case. A probability inherits the log-sum's error
 and its own t's: (350 + 4 + 3 |t|) 2^-24 relative."""
 import math
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -378,6 +381,58 @@ def test_streamed_rows_against_single_rows(shape):
         assert (out.grad[dead] == 0).all() and (out.logprob[dead] == 0).all() and (out.row_loss[dead] == 0).all()
 
 
+@pytest.mark.parametrize("shape", [(6, 300), (600, 30001)], ids=str)
+def test_clipped_rows(shape):
+    """A clipped ratio without KL term and bonus: a gradient of zeros, the clipped loss."""
+    rows, V = shape
+    logits, targets, g = rows_of(rows, V, torch.float32, 62)
+    lp, _ = reference(logits, targets, 1.0)
+    up = torch.arange(rows, device="cuda") % 2 == 0
+    old = (lp - torch.where(up, 1.0, -1.0)).float()          # ratios of e and 1/e
+    adv = torch.where(up, 1.0, -1.0).float().contiguous()     # out of the range on the side that is clipped
+    adv[rows // 2:] *= -1                                     # ... and on the side that is not
+    out = q().policy_loss(logits, targets, old, adv, weight=torch.ones(rows, device="cuda"))
+    clipped = torch.arange(rows, device="cuda") < rows // 2
+    assert (out.grad[clipped] == 0).all()
+    assert (out.grad[~clipped].abs().amax(1) > 0).all()
+    want = torch.where(up, -1.2, 0.8).float()                 # fp32 borders: half a step each
+    assert (out.row_loss[clipped] - want[clipped]).abs().max() <= 2.0 ** -23
+
+
+def test_two_streamed_calls_at_once():
+    """Two calls of the streaming kernel on two streams, each holding SMs that the other waits for."""
+    rows, V = 600, 30001
+    sets = [policy_inputs(rows, V, 0, 0, 1.0, 0.2, 0.2, torch.float32, 70 + i, True) for i in range(2)]
+    call = lambda s, **kw: q().policy_loss(s[0], s[1], s[2], s[3], weight=s[5], entropy_coef=0.01, **kw)  # noqa: E731
+    want = [call(s) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[call(s, stream=st) for s, st in zip(sets, streams)] for _ in range(4)]
+    torch.cuda.synchronize()
+    for turn in got:
+        for a, b in zip(turn, want):
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_first_calls_under_capture():
+    """A process whose first calls are captured, without a call before that sets the kernels up."""
+    code = """
+import torch, quasar_b200 as q
+l = torch.randn(600, 30001, device='cuda'); t = torch.zeros(600, dtype=torch.int32, device='cuda'); f = torch.full((600,), -9.0, device='cuda')
+cu = torch.tensor([0, 300, 600], dtype=torch.int32, device='cuda')
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    a, b, c = q.policy_loss(l, t, f, f, entropy_coef=0.1), q.preference_loss(l, t, cu), q.token_logprobs(l, t)
+g.replay()
+torch.cuda.synchronize()
+x, y, z = q.policy_loss(l, t, f, f, entropy_coef=0.1), q.preference_loss(l, t, cu), q.token_logprobs(l, t)
+same = lambda m, n: all(torch.equal(i, j) for i, j in zip(m, n) if i is not None)
+assert same(a, x) and same(b, y) and same(c, z)
+"""
+    subprocess.run([sys.executable, "-c", code], check=True, timeout=300, cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+
+
 def test_more_rows_than_one_launch_takes():
     """Batches beyond 16384 streamed rows: every row as in a batch of its own half."""
     rows, V = 16500, 50021
@@ -455,6 +510,20 @@ def test_preference_loss(dtype, case):
     over = q().preference_loss(again, targets, cu, ref_logprob=ref, pair_weight=w, temperature=T, beta=beta,
                                label_smoothing=eps, length_normalize=mean, grad_scale=32.0, grad=again, out=out)
     assert torch.equal(over.grad, out.grad)
+
+
+def test_infinite_preferences():
+    """A chosen sequence of probability 0: an infinite loss, but with the pair turned round (label_smoothing 1) none;
+    the gradient stays finite."""
+    logits, targets, g = rows_of(4, 50, torch.float32, 33)
+    logits[1, targets[1]] = -math.inf
+    cu = torch.tensor([0, 2, 4], dtype=torch.int32, device="cuda")
+    out = q().preference_loss(logits, targets, cu)
+    assert out.loss.item() == math.inf and out.seq_logprob[0].item() == -math.inf
+    assert torch.isfinite(out.grad).all()
+    assert torch.allclose(out.row_grad, torch.tensor([-0.1, -0.1, 0.1, 0.1], device="cuda"), rtol=1e-6)
+    out = q().preference_loss(logits, targets, cu, label_smoothing=1.0)
+    assert out.loss.item() == 0 and (out.grad == 0).all()
 
 
 def test_preference_offsets_that_leave_the_rows():
