@@ -119,15 +119,14 @@ __device__ __forceinline__ Span span_of(const T* row, int V) {
 
 
 // Part `part` of `parts` of a row's packs, and the edge element (of part 0)
-// that this thread takes: at most 2 * (N - 1) of them, one a thread.
+// that thread tid takes: at most 2 * (N - 1) of them, one a thread.
 struct Slice {
     int head, lo, n;  // packs [lo, lo + n)
     int edge;         // element, or -1
 };
 template <typename T>
-__device__ __forceinline__ Slice slice_of(const T* row, int V, int part, int parts) {
+__device__ __forceinline__ Slice slice_of(const T* row, int V, int part, int parts, int tid) {
     const Span sp = span_of(row, V);
-    const int tid = threadIdx.x;
     Slice s;
     s.head = sp.head;
     s.lo = (int)((unsigned)sp.packs * (unsigned)part / (unsigned)parts);
@@ -474,13 +473,13 @@ __device__ __forceinline__ void put_edge(T* out, int v, int target, float l, con
 // wide rows, fills, and rows of another 16-byte phase than the logits'.
 // Packs [lo, hi), pack lo + i by thread i % nt.
 template <typename T, bool ENT>
-__device__ __noinline__ void grad_plain(const T* row, T* out, int head, int lo, int hi, Coef c, float k, int nt) {
+__device__ __noinline__ void grad_plain(const T* row, T* out, int head, int lo, int hi, Coef c, float k, int tid, int nt) {
     const uint4* src = reinterpret_cast<const uint4*>(row + head);
     T* dst = out + head;
     const bool same = ((uintptr_t)dst & 15) == 0;
     const uint4 fill = fill_pack<T>(c);
 #pragma unroll 4
-    for (int v = lo + (int)threadIdx.x; v < hi; v += nt) {
+    for (int v = lo + tid; v < hi; v += nt) {
         uint4 g = fill;
         if (elementwise(c)) {
             const uint4 p = load_pack(src + v);
@@ -521,7 +520,7 @@ __device__ __forceinline__ void remote_store(uint32_t addr, const Part& p) {
 // that l * k overflows (a row masked throughout by the type's lowest value).
 template <typename T, bool ENT>
 __device__ __noinline__ Part wide_part(const T* row, int V, float M, float k, int part, int parts, int first, int nt) {
-    const Slice sl = slice_of(row, V, part, parts);
+    const Slice sl = slice_of(row, V, part, parts, 0);
     const int v0 = part == 0 ? 0 : sl.head + sl.lo * Type<T>::N, v1 = part == parts - 1 ? V : sl.head + (sl.lo + sl.n) * Type<T>::N;
     float s = 0.0f, q = 0.0f;
 #pragma unroll 4
@@ -561,21 +560,40 @@ __device__ __forceinline__ void wait_before() { asm volatile("griddepcontrol.wai
 // Measured at V = 151936: 8191 bf16 rows, a tenth of them left out, in 325 us
 // (1.05 of the measured copy rate: reads are a little faster than copies); one fp32
 // row in 6.2 us.
-template <typename T, bool ENT, bool POLICY, int NT>
-__global__ void __launch_bounds__(NT, 1024 / NT) rows_kernel(const Args a) {
+// With ROWS > 1 (NT = 32) a CTA's warps take a row each: short rows by CTAs of
+// one warp are bound by the rate at which CTAs start, 2.1 ns each (20000 f16
+// rows of 1000 columns: 47.6 us with one row a CTA, 15.9 with 8).
+template <typename T, bool ENT, bool POLICY, int NT, int ROWS>
+__global__ void __launch_bounds__(NT * ROWS, 1024 / (NT * ROWS)) rows_kernel(const Args a) {
+    static_assert(ROWS == 1 || NT == 32, "a row for each warp, or the CTA's threads for one row");
     constexpr int N = Type<T>::N, NW = NT / 32, STEP = NT * U;
-    __shared__ Part parts[2][MAXC * NW];
-    __shared__ Coef coef;
-    __shared__ bool again;
-    __shared__ float wide_m;
-    const int C = (int)cluster_size(), rank = (int)cluster_rank();
-    const int64_t r = blockIdx.x / C;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    __shared__ Part parts_of[ROWS][2][MAXC * NW];
+    __shared__ Coef coef_of[ROWS];
+    __shared__ bool again_of[ROWS];
+    __shared__ float wide_m_of[ROWS];
+    const int C = ROWS == 1 ? (int)cluster_size() : 1, rank = ROWS == 1 ? (int)cluster_rank() : 0;
+    const int group = ROWS == 1 ? 0 : (int)threadIdx.x / NT;
+    const int tid = ROWS == 1 ? (int)threadIdx.x : (int)threadIdx.x % NT, lane = tid & 31, warp = tid >> 5;
+    const int64_t r = ROWS == 1 ? (int64_t)(blockIdx.x / C) : (int64_t)blockIdx.x * ROWS + group;
+    if (ROWS > 1 && r >= a.rows) {
+        launch_next();
+        return;
+    }
+    Part(&parts)[2][MAXC * NW] = parts_of[group];
+    Coef& coef = coef_of[group];
+    bool& again = again_of[group];
+    float& wide_m = wide_m_of[group];
+    const auto sync = [] {
+        if (ROWS == 1)
+            __syncthreads();
+        else
+            __syncwarp();
+    };
     const T* row = (const T*)a.logits + r * a.ld;
     const float k = a.k;
     const int target = a.targets[r];
     const double weight = POLICY ? (a.weight ? (double)a.weight[r] : a.mean) : 1.0;
-    const Slice s = slice_of(row, a.V, rank, C);
+    const Slice s = slice_of(row, a.V, rank, C, tid);
     const uint4* src = reinterpret_cast<const uint4*>(row + s.head) + s.lo + tid;
     // the first batch is the ragged one, and on its way before the row is known to take part
     int first = s.n % STEP;
@@ -597,7 +615,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) rows_kernel(const Args a) {
         if (POLICY && a.grad) {
             const Coef c = fill_coef(live);
             if (s.edge >= 0) put_edge<T, ENT>(out, s.edge, target, 0.0f, c, k);
-            grad_plain<T, ENT>(row, out, s.head, s.lo, s.lo + s.n, c, k, NT);
+            grad_plain<T, ENT>(row, out, s.head, s.lo, s.lo + s.n, c, k, tid, NT);
         }
         return;
     }
@@ -630,7 +648,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) rows_kernel(const Args a) {
             cluster_wait();
         } else {
             if (lane == 0) parts[turn][warp] = mine;
-            __syncthreads();
+            sync();
         }
         if (warp == 0) {
             const Row w = turn ? join_wide(parts[1], C * NW, wide, k) : join_parts<ENT>(parts[0], C * NW, k);
@@ -638,11 +656,11 @@ __global__ void __launch_bounds__(NT, 1024 / NT) rows_kernel(const Args a) {
             if (turn || !w.wide) c = finish_row<ENT, POLICY>(a, r, w, in, rank == 0 && lane == 0);
             if (lane == 0) coef = c, again = !turn && w.wide, wide_m = w.M;
         }
-        __syncthreads();
+        sync();
         if (!again) break;
         wide = wide_m;
         mine = wide_part<T, ENT>(row, a.V, wide, k, rank, C, tid, NT);
-        __syncthreads();  // again and wide_m are written once more
+        sync();  // again and wide_m are written once more
     }
     launch_next();
     if (!POLICY || !a.grad) return;
@@ -674,7 +692,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) rows_kernel(const Args a) {
         }
         if (hot >= first) hot_thread = (hot - first) % NT;  // batches begin at first + i * STEP
     } else {
-        grad_plain<T, ENT>(row, out, s.head, s.lo, s.lo + s.n, c, k, NT);
+        grad_plain<T, ENT>(row, out, s.head, s.lo, s.lo + s.n, c, k, tid, NT);
     }
     // the thread that wrote the target's pack puts the target right
     if (hot >= 0 && hot < s.n && tid == hot_thread && elementwise(c)) put1(out + target, grad1<ENT>(c, c.lt, k) + c.one);
@@ -847,7 +865,7 @@ __global__ void __launch_bounds__(Shape::NT + 64, Shape::CTAS) stream_kernel(con
                 if (i < mine_n) {
                     const int64_t r = nth_row(sh, a.rows, cid + i * step, false);
                     const T* row = (const T*)a.logits + r * a.ld;
-                    const Slice s = slice_of(row, a.V, rank, C);
+                    const Slice s = slice_of(row, a.V, rank, C, tid);
                     src = reinterpret_cast<const uint4*>(row + s.head) + s.lo;
                     packs = s.n, n = (s.n + CHP - 1) / CHP;
                     sh.rows[i & 7] = (int)r;
@@ -942,7 +960,7 @@ __global__ void __launch_bounds__(Shape::NT + 64, Shape::CTAS) stream_kernel(con
                 stream_wait(full_u + 8 * stage, phase, abort);
                 r = *abort ? nth_row(sh, a.rows, cid + i * step, false) : *(volatile int*)&sh.rows[i & 7];
                 row = (const T*)a.logits + r * a.ld;
-                s = slice_of(row, a.V, rank, C);
+                s = slice_of(row, a.V, rank, C, tid);
                 n = (s.n + CHP - 1) / CHP;
                 if (s.edge >= 0) edge = widen1(row[s.edge]);
             }
@@ -1036,10 +1054,10 @@ __global__ void __launch_bounds__(Shape::NT + 64, Shape::CTAS) stream_kernel(con
             if (tid == 0) blank_row<true>(a, r, nan ? NAN : 0.0f);
             const T* row = (const T*)a.logits + r * a.ld;
             T* out = (T*)a.grad + r * a.grad_ld;
-            const Slice s = slice_of(row, a.V, 0, 1);
+            const Slice s = slice_of(row, a.V, 0, 1, tid);
             const Coef c = fill_coef(nan);
             if (s.edge >= 0) put_edge<T, ENT>(out, s.edge, target, 0.0f, c, k);
-            grad_plain<T, ENT>(row, out, s.head, 0, s.n, c, k, NT);
+            grad_plain<T, ENT>(row, out, s.head, 0, s.n, c, k, tid, NT);
         }
     }
     // no CTA leaves while a peer may still store into its shared memory
@@ -1055,19 +1073,23 @@ __global__ void __launch_bounds__(Shape::NT + 64, Shape::CTAS) stream_kernel(con
 // Measured: 2047 bf16 rows of 151936, a fifth of them zeros, in 177 us (0.97
 // of the measured copy rate) with slices of 76 KB; slices of a quarter of
 // that, in which a CTA's start weighs more, take 234 us.
-template <typename T, bool ENT>
+// ROWS > 1: a warp for each row, for short ones (20000 f16 rows of 1000
+// columns: 56 us with a CTA for each, 20 with a warp).
+template <typename T, bool ENT, int ROWS>
 __global__ void __launch_bounds__(256, 6) grad_kernel(const Args a, const int parts) {
-    constexpr int N = Type<T>::N, NT = 256;
+    constexpr int N = Type<T>::N, NT = 256 / ROWS;
     wait_before();
-    const int64_t r = blockIdx.x / (unsigned)parts;
-    const int part = (int)(blockIdx.x - (unsigned)r * (unsigned)parts);
+    const int tid = ROWS == 1 ? (int)threadIdx.x : (int)threadIdx.x % NT;
+    const int64_t r = ROWS == 1 ? (int64_t)(blockIdx.x / (unsigned)parts) : (int64_t)blockIdx.x * ROWS + threadIdx.x / NT;
+    if (ROWS > 1 && r >= a.rows) return;
+    const int part = ROWS == 1 ? (int)(blockIdx.x - (unsigned)r * (unsigned)parts) : 0;
     const float k = a.k;
     const int target = a.targets[r];
     const float g_lp = a.g_lp[r], g_ent = ENT ? a.g_ent[r] : 0.0f, ent = ENT ? a.ent_in[r] : 0.0f;
     const quasar_logprob_stat st = a.stats_in[r];
     const T* row = (const T*)a.logits + r * a.ld;
     T* out = (T*)a.grad + r * a.grad_ld;
-    const Slice s = slice_of(row, a.V, part, parts);
+    const Slice s = slice_of(row, a.V, part, ROWS == 1 ? parts : 1, tid);
     Coef c = fill_coef(target >= a.V);
     if (target >= 0 && target < a.V) {
         const float R = st.max * k;
@@ -1077,14 +1099,14 @@ __global__ void __launch_bounds__(256, 6) grad_kernel(const Args a, const int pa
         c = make_coef(st.max, R, wide, S, ENT ? ent - logf(S) : 0.0f, g_lp, g_ent, (float)a.inv_t);
     }
     const int hot = target >= s.head ? (target - s.head) / N - s.lo : -1;
-    const bool mine = elementwise(c) && hot >= 0 && hot < s.n && hot % NT == (int)threadIdx.x;
+    const bool mine = elementwise(c) && hot >= 0 && hot < s.n && hot % NT == tid;
     const float lt = mine ? widen1(row[target]) : 0.0f;  // read before its pack is written over
     if (s.edge >= 0) put_edge<T, ENT>(out, s.edge, target, elementwise(c) ? widen1(row[s.edge]) : 0.0f, c, k);
-    const uint4* src = reinterpret_cast<const uint4*>(row + s.head) + s.lo + threadIdx.x;
-    T* dst = out + s.head + (int64_t)(s.lo + (int)threadIdx.x) * N;
+    const uint4* src = reinterpret_cast<const uint4*>(row + s.head) + s.lo + tid;
+    T* dst = out + s.head + (int64_t)(s.lo + tid) * N;
     if (((uintptr_t)dst & 15) == 0 && c.kind == ROW_SUM) {
         uint4* d = reinterpret_cast<uint4*>(dst);
-        const int n = s.n - (int)threadIdx.x;
+        const int n = s.n - tid;
         int v = 0;
         for (; v + (U - 1) * NT < n; v += NT * U) {
             uint4 p[U];
@@ -1101,7 +1123,7 @@ __global__ void __launch_bounds__(256, 6) grad_kernel(const Args a, const int pa
         for (int u = 0; u < U; u++)
             if (v + u * NT < n) d[v + u * NT] = grad_of<T, ENT>(p[u], c, k);
     } else {
-        grad_plain<T, ENT>(row, out, s.head, s.lo, s.lo + s.n, c, k, NT);
+        grad_plain<T, ENT>(row, out, s.head, s.lo, s.lo + s.n, c, k, tid, NT);
     }
     if (mine) put1(out + target, grad1<ENT>(c, lt, k) + c.one);
 }
@@ -1164,20 +1186,21 @@ __global__ void __launch_bounds__(128) pair_kernel(const PairArgs p) {
                 if (p.targets[r] >= 0) p.row_grad[r] = (float)((s ? -g : g) * by[s]);
 }
 
-// One CTA: the same order of sums in every run.
-__global__ void __launch_bounds__(512) weighted_sum_kernel(const float* x, const float* w, int n, float* out) {
-    __shared__ double buf[16];
+// One CTA: the same order of sums in every run. A weight of 0 takes nothing,
+// of an infinite x either.
+__global__ void __launch_bounds__(1024) weighted_sum_kernel(const float* x, const float* w, int n, float* out) {
+    __shared__ double buf[32];
     wait_before();
     launch_next();
     double s = 0.0;
-    for (int64_t i = threadIdx.x; i < n; i += 512) {
-        const double wi = w ? (double)w[i] : 1.0;
-        if (wi != 0.0) s += wi * (double)x[i];
+#pragma unroll 8
+    for (int64_t i = threadIdx.x; i < n; i += 1024) {
+        const float wi = w ? w[i] : 1.0f, xi = x[i];
+        s += wi != 0.0f ? (double)wi * (double)xi : 0.0;
     }
-    s = cta_sum(s, buf, 512);
+    s = cta_sum(s, buf, 1024);
     if (threadIdx.x == 0) out[0] = (float)(w || n == 0 ? s : s / n);
 }
-
 
 // ---- launchers ---------------------------------------------------------------
 
@@ -1219,10 +1242,16 @@ static int row_cluster(int64_t rows, int64_t row_bytes) {
     return C;
 }
 
-template <typename T, bool ENT, bool POLICY, int NT>
+template <typename T, bool ENT, bool POLICY, int NT, int ROWS>
 static cudaError_t rows_launch(const Args& a, int C, cudaStream_t st) {
-    return launch(rows_kernel<T, ENT, POLICY, NT>, (unsigned)a.rows * (unsigned)C, NT, 0, C, false, st, a);
+    const unsigned grid = ((unsigned)a.rows + ROWS - 1) / ROWS * (unsigned)C;
+    return launch(rows_kernel<T, ENT, POLICY, NT, ROWS>, grid, NT * ROWS, 0, ROWS == 1 ? C : 0, false, st, a);
 }
+
+// Rows that a warp takes alone, in bytes: 20000 bf16 rows of 4000 columns,
+// policy loss and gradient, 80 us against 110 with 128 threads a row; 500 rows
+// of 18 KB 13.1 against 9.4.
+static constexpr int64_t ROW_SHORT = 8192;
 
 // Short rows take small CTAs, of which an SM runs more at once: a CTA's start,
 // its barrier and its scalars take about 4 us whatever its slice. bf16 rows of
@@ -1232,9 +1261,9 @@ template <typename T, bool ENT, bool POLICY>
 static cudaError_t rows_by_size(const Args& a, cudaStream_t st) {
     const int64_t row_bytes = (int64_t)a.V * sizeof(T);
     const int C = row_cluster(a.rows, row_bytes);
-    if (C == 1 && row_bytes <= 4096) return rows_launch<T, ENT, POLICY, 32>(a, C, st);
-    if (C == 1 && row_bytes <= 49152) return rows_launch<T, ENT, POLICY, 128>(a, C, st);
-    return rows_launch<T, ENT, POLICY, 256>(a, C, st);
+    if (C == 1 && row_bytes <= ROW_SHORT) return rows_launch<T, ENT, POLICY, 32, 8>(a, C, st);
+    if (C == 1 && row_bytes <= 49152) return rows_launch<T, ENT, POLICY, 128, 1>(a, C, st);
+    return rows_launch<T, ENT, POLICY, 256, 1>(a, C, st);
 }
 
 // Long rows: one CTA of 640 consumers per SM with chunks of 30 KB. Middle
@@ -1329,12 +1358,17 @@ cudaError_t launch_rows(const Args& a, int dtype, cudaStream_t st) {
 template <typename T>
 static cudaError_t grad_typed(const Args& a, cudaStream_t st) {
     const int64_t row_bytes = (int64_t)a.V * sizeof(T);
+    if (row_bytes <= ROW_SHORT) {
+        const unsigned grid = ((unsigned)a.rows + 7) / 8;
+        if (a.g_ent) return launch(grad_kernel<T, true, 8>, grid, 256, 0, 0, true, st, a, 1);
+        return launch(grad_kernel<T, false, 8>, grid, 256, 0, 0, true, st, a, 1);
+    }
     int64_t parts = (row_bytes + 77823) / 77824;
     while (parts * a.rows < 4 * SMS && row_bytes > parts * 2 * 8192) parts *= 2;
     if (parts * a.rows > INT32_MAX) parts = 1;
     const unsigned grid = (unsigned)(a.rows * parts);
-    if (a.g_ent) return launch(grad_kernel<T, true>, grid, 256, 0, 0, true, st, a, (int)parts);
-    return launch(grad_kernel<T, false>, grid, 256, 0, 0, true, st, a, (int)parts);
+    if (a.g_ent) return launch(grad_kernel<T, true, 1>, grid, 256, 0, 0, true, st, a, (int)parts);
+    return launch(grad_kernel<T, false, 1>, grid, 256, 0, 0, true, st, a, (int)parts);
 }
 
 cudaError_t launch_grad(const Args& a, int dtype, cudaStream_t st) {
@@ -1346,7 +1380,7 @@ cudaError_t launch_grad(const Args& a, int dtype, cudaStream_t st) {
 cudaError_t launch_pairs(const PairArgs& p, cudaStream_t st) { return launch(pair_kernel, (unsigned)p.pairs, 128, 0, 0, true, st, p); }
 
 cudaError_t launch_weighted_sum(const float* x, const float* w, int n, float* out, cudaStream_t st) {
-    return launch(weighted_sum_kernel, 1u, 512, 0, 0, true, st, x, w, n, out);
+    return launch(weighted_sum_kernel, 1u, 1024, 0, 0, true, st, x, w, n, out);
 }
 
 }  // namespace loss

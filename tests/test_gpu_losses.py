@@ -346,10 +346,11 @@ def special_rows(logits, targets):
     return [6, 7, 8]
 
 
-@pytest.mark.parametrize("shape", [(600, 50021, torch.float16), (160, 40001, torch.float32), (300, 151936, torch.bfloat16)], ids=str)
-def test_streamed_rows_against_single_rows(shape):
-    """The streaming kernel takes many long rows, a cluster per row a few: the same rows either way, masks of every
-    kind and rows that take no part among them. Both are within the bounds above of the exact values, and so within
+@pytest.mark.parametrize("shape", [(600, 50021, torch.float16), (160, 40001, torch.float32), (300, 151936, torch.bfloat16),
+                                   (321, 1001, torch.float32), (403, 3001, torch.bfloat16), (330, 9001, torch.float16)], ids=str)
+def test_many_rows_against_few(shape):
+    """The streaming kernel takes many long rows, a warp or a small CTA each of many short ones, a cluster each of
+    few: the same rows either way, masks of every kind and rows that take no part among them. Both are within the bounds above of the exact values, and so within
     twice of each other; coefficients are rounded from sums that differ by those bounds, not more."""
     rows, V, dtype = shape
     logits, targets, old, adv, ref, w = policy_inputs(rows, V, 0, 0, 1.0, 0.2, 0.2, dtype, 60, True)
