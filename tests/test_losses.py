@@ -40,7 +40,8 @@ def policy(prm=(1.0, 0.2, 0.2, 0.0, 0.0, 1.0), **kw):
     a = dict(logits=P(4096), dtype=0, ld=16, rows=2, V=16, targets=P(64), old=P(64), adv=P(64), ref=None, weight=None,
              logprob=P(64), entropy=None, row_loss=P(64), loss=P(64), grad=P(8192), grad_ld=16)
     a.update(kw)
-    p = None if prm is None else ctypes.addressof(PolicyParams(*prm))
+    rec = None if prm is None else PolicyParams(*prm)
+    p = None if rec is None else ctypes.addressof(rec)
     return _lib().quasar_policy_loss(a["logits"], a["dtype"], a["ld"], a["rows"], a["V"], a["targets"], a["old"],
                                      a["adv"], a["ref"], a["weight"], p, a["logprob"], a["entropy"], a["row_loss"],
                                      a["loss"], a["grad"], a["grad_ld"], None)
@@ -52,7 +53,8 @@ def preference(prm=(1.0, 0.1, 0.0, 1.0, 0, 0), **kw):
              logprob=P(64), seq=P(64), pair_loss=P(64), loss=P(64), stats=P(64), row_grad=P(64), grad=P(8192),
              grad_ld=16)
     a.update(kw)
-    p = None if prm is None else ctypes.addressof(PreferenceParams(*prm))
+    rec = None if prm is None else PreferenceParams(*prm)
+    p = None if rec is None else ctypes.addressof(rec)
     return _lib().quasar_preference_loss(a["logits"], a["dtype"], a["ld"], a["rows"], a["V"], a["targets"], a["cu"],
                                          a["pairs"], a["ref"], a["weight"], p, a["logprob"], a["seq"], a["pair_loss"],
                                          a["loss"], a["stats"], a["row_grad"], a["grad"], a["grad_ld"], None)
