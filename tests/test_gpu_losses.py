@@ -453,6 +453,9 @@ PAIRS = [  # lengths, rows behind, V, T, beta, smoothing, mean, with reference
     ([0, 3, 5, 0, 0, 0], 1, 260, 0.7, 0.5, 0.0, True, True), ([17, 9, 200, 150], 0, 4099, 1.0, 0.05, 0.2, False, True),
     ([4, 5, 2, 7], 3, 18992, 1.0, 2.0, 0.0, True, False), ([3, 2], 0, 151936, 1.0, 0.1, 1.0, False, True),
     ([2, 1] * 150, 5, 97, 1.0, 0.2, 0.0, False, True),
+    # batches beyond L2, with long, short and empty sequences
+    ([100, 90, 400, 300, 0, 5, 250, 255, 1, 1, 600, 100, 0, 0, 3, 2], 7, 30001, 1.0, 0.02, 0.1, False, True),
+    ([2, 3] * 420, 0, 30001, 0.9, 0.5, 0.0, True, False),
 ]
 
 
