@@ -29,10 +29,9 @@
  *   p_v      = exp((l_v - M) / temperature) / S
  *   logprob  = (l_target - M) / temperature - ln S
  *   entropy  = -sum p ln p
- * Sums are kept in 32 bits within a warp and in 64 bits across warps; a
- * log-probability is formed in 64 bits from them and rounded once, the
- * exponentials of its differences (ratio, KL term) in 32 bits; gradients are
- * formed in 32 bits and rounded once to dtype. A row whose derivatives by
+ * Sums are kept in 32 bits within a warp and in 64 bits across warps;
+ * log-probabilities, entropies and losses are formed in 64 bits from them and
+ * rounded once; gradients are formed in 32 bits and rounded once to dtype. A row whose derivatives by
  * log-probability and entropy are both 0 (a clipped ratio) has a gradient of
  * zeros, whatever its logits. */
 #ifndef QUASAR_LOSSES_H

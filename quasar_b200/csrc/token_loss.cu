@@ -2,8 +2,8 @@
 // made of them (include/quasar_losses.h).
 //
 // The mathematics: with k = log2(e) / T, M the largest logit of a row, R = M*k
-// rounded to fp32 and t = l*k - R (one fused multiply-add), the row's softmax
-// needs S = sum 2^t and its entropy also Q = sum 2^t * t:
+// rounded to a whole number and t = l*k - R (one fused multiply-add), the row's
+// softmax needs S = sum 2^t and its entropy also Q = sum 2^t * t:
 //   logprob = ln2 * t_target - ln S,  entropy = ln S - ln2 * Q / S,
 //   p_v = 2^t / S.
 // M is not known while the row streams, so a thread sums against a reference
@@ -191,7 +191,7 @@ template <bool ENT>
 __device__ __forceinline__ void acc_raise(Acc& a, float mx, float k) {
     a.mx = fmaxf(a.mx, mx);
     if (fmaf(mx, k, -a.c) > LAG) {
-        const float c = mx * k, d = fmaxf(a.c - c, -1e30f);  // finite, for sums still at 0
+        const float c = rintf(mx * k), d = fmaxf(a.c - c, -1e30f);  // finite, for sums still at 0
         const float f = ex2_approx(d);
         const f32x2 ff = pack2(f, f);
         if (ENT) a.q = mul2(fma2(a.s, pack2(d, d), a.q), ff);
@@ -240,7 +240,7 @@ struct __align__(16) Part {
 
 // The reference of sums with maximum m (finite for a maximum of the lowest
 // value or -inf, whose sums are 0).
-__device__ __forceinline__ float scaled(float m, float k) { return fmaxf(m * k, NEG); }
+__device__ __forceinline__ float scaled(float m, float k) { return fmaxf(rintf(m * k), NEG); }
 
 // Brings sums taken against the scaled reference `from` to the one of `m`.
 __device__ __forceinline__ void rebase(float& s, float& q, float from, float m, float k) {
@@ -332,57 +332,76 @@ struct RowIn {  // a row's inputs beside its logits
     double weight;
 };
 
-// ln S for S >= 1 (or 0, NaN) to about 1e-7 absolute: the exponent's part in
-// 64 bits, the mantissa's by logf on [1, 2).
+// ln S to about 3e-8 absolute: the exponent's part in 64 bits, the mantissa's
+// by logf on [1, 2).
 __device__ __forceinline__ double ln_sum(double S) {
     const float s = (float)S;
-    const int e = ((__float_as_int(s) >> 23) & 255) - 127;
     if (!(s > 1e-30f && s < 1e30f)) return (double)logf(s);
+    const int e = ((__float_as_int(s) >> 23) & 255) - 127;
     const float m = __int_as_float((__float_as_int(s) & 0x007FFFFF) | 0x3F800000);
     // the rounding of S to s goes in to first order
-    return e * LN2 + (double)(logf(m) + (float)((S - (double)s)) / s);
+    return e * LN2 + (double)(logf(m) + (float)(S - (double)s) / s);
 }
 
-// Writes a row's outputs (one thread) and returns its gradient's
-// coefficients. The log-probability is formed in 64 bits; the exponentials of
-// its differences, which are near 1, are expf's (2^-23 relative): their
-// 64-bit forms took 1.4 us on the path between the row's two passes.
-template <bool ENT, bool POLICY>
-__device__ __forceinline__ Coef finish_row(const Args& a, int64_t r, const Row& w, const RowIn& in, bool write) {
-    const bool none = w.M == -INFINITY && w.S == 0.0;
-    const double lnS = ln_sum(w.S);
-    const double lp = none ? -INFINITY : ((double)in.lt * (double)a.k - w.R) * LN2 - lnS;
-    const float S = (float)w.S;
-    const float h_ln_s = ENT && !none ? (float)-LN2 * ((float)w.Q / S) : 0.0f;
-    const float H = ENT && !none ? (float)(lnS + (double)h_ln_s) : 0.0f;
-    float loss = 0.0f;
-    Coef c = fill_coef(false);
-    if (POLICY) {
-        const float adv = in.adv, ratio = expf((float)(lp - (double)in.old_lp));
-        const float lo = (float)(1.0 - a.clip_lo), hi = (float)(1.0 + a.clip_hi);
-        const float fit = ratio < lo ? lo : ratio > hi ? hi : ratio;  // NaN stays
-        const float x = ratio * adv, y = fit * adv;
-        loss = x <= y ? -x : y < x ? -y : NAN;
-        float g = x <= y ? -x : y < x ? 0.0f : NAN;
-        if (a.kl != 0.0) {
-            const float u = (float)((double)in.ref_lp - lp), eu = expm1f(u);
-            loss += (float)a.kl * (isinf(eu) ? eu : eu - u);
-            g -= (float)a.kl * eu;
-        }
-        if (ENT && a.ec != 0.0) loss -= (float)a.ec * H;
-        g *= (float)(in.weight * a.scale);
-        if (a.grad) c = make_coef(w.M, (float)w.R, w.wide, S, h_ln_s, g, ENT ? (float)(-a.ec * in.weight * a.scale) : 0.0f, (float)a.inv_t);
-        c.lt = in.lt;
-    }
-    if (write) {
-        a.logprob[r] = (float)lp;
-        if (a.entropy) a.entropy[r] = H;
-        // S was summed against R, the rounded M * k
-        if (a.stats) a.stats[r] = {w.M, S * (none ? 1.0f : ex2_approx((float)(w.R - (double)w.M * (double)a.k)))};
-        if (a.row_grad) a.row_grad[r] = 0.0f;
-        if (POLICY) a.row_loss[r] = loss;
-    }
+// The log-probability (-inf: no distribution, or none on the target), not
+// above 0 by the terms' errors either.
+__device__ __forceinline__ double row_logprob(const Args& a, const Row& w, float lt) {
+    if (w.M == -INFINITY && w.S == 0.0) return -INFINITY;
+    const double lp = ((double)lt * (double)a.k - w.R) * LN2 - ln_sum(w.S);
+    return lp > 0.0 ? 0.0 : lp;
+}
+
+// The policy loss's derivative by the row's log-probability. F: the precision;
+// a ratio at a border counts as not clipped.
+template <typename F>
+__device__ __forceinline__ F policy_slope(const Args& a, F adv, F ratio, F eu, F* loss) {
+    const F lo = (F)(1.0 - a.clip_lo), hi = (F)(1.0 + a.clip_hi);
+    const F fit = ratio < lo ? lo : ratio > hi ? hi : ratio;  // NaN stays
+    const F x = ratio * adv, y = fit * adv;
+    *loss = x <= y ? -x : y < x ? -y : (F)NAN;
+    return (x <= y ? -x : y < x ? (F)0 : (F)NAN) - (a.kl != 0.0 ? (F)a.kl * eu : (F)0);
+}
+
+// A row's gradient coefficients. All the row's threads wait for them, so the
+// exponentials of differences of log-probabilities, which are near 1, are
+// expf's here (2^-23 relative); their 64-bit forms took 1.4 us.
+template <bool ENT>
+__device__ __forceinline__ Coef row_coef(const Args& a, const Row& w, const RowIn& in) {
+    const double lp = row_logprob(a, w, in.lt);
+    const float S = (float)w.S, ratio = expf((float)(lp - (double)in.old_lp));
+    const float eu = a.kl != 0.0 ? expm1f((float)((double)in.ref_lp - lp)) : 0.0f;
+    float loss;
+    const float ws = (float)(in.weight * a.scale), g = policy_slope<float>(a, in.adv, ratio, eu, &loss) * ws;
+    Coef c = make_coef(w.M, (float)w.R, w.wide, S, ENT ? (float)-LN2 * ((float)w.Q / S) : 0.0f, g, ENT ? -(float)a.ec * ws : 0.0f, (float)a.inv_t);
+    c.lt = in.lt;
     return c;
+}
+
+// Writes a row's outputs (one thread of the calling warp). The loss is formed
+// in 64 bits: a mean over rows of either sign keeps little of each.
+template <bool ENT, bool POLICY>
+__device__ __forceinline__ void write_row(const Args& a, int64_t r, const Row& w, const RowIn& in) {
+    const bool none = w.M == -INFINITY && w.S == 0.0;
+    const double lp = row_logprob(a, w, in.lt);
+    double H = 0.0;
+    if (ENT && !none) {
+        const float S = (float)w.S, q = (float)w.Q / S;
+        H = ln_sum(w.S) - LN2 * ((double)q + (double)((float)(w.Q - (double)q * w.S) / S));
+        if (H < 0.0) H = 0.0;
+    }
+    a.logprob[r] = (float)lp;
+    if (a.entropy) a.entropy[r] = (float)H;
+    // S was summed against R, not M * k
+    if (a.stats) a.stats[r] = {w.M, (float)(w.S * (none ? 1.0 : exp2(w.R - (double)w.M * (double)a.k)))};
+    if (a.row_grad) a.row_grad[r] = 0.0f;
+    if (POLICY) {
+        const double u = a.kl != 0.0 ? (double)in.ref_lp - lp : 0.0, eu = a.kl != 0.0 ? expm1(u) : 0.0;
+        double loss;
+        policy_slope<double>(a, in.adv, exp(lp - (double)in.old_lp), eu, &loss);
+        if (a.kl != 0.0) loss += a.kl * (isinf(eu) ? eu : eu - u);
+        if (ENT && a.ec != 0.0) loss -= a.ec * H;
+        a.row_loss[r] = (float)loss;
+    }
 }
 
 // Outputs of a row that takes no part (0) or whose target is out of range (NaN).
@@ -639,6 +658,7 @@ __global__ void __launch_bounds__(NT * ROWS, 1024 / (NT * ROWS)) rows_kernel(con
     acc_packs<T, ENT>(acc, p, k);
     if (s.edge >= 0) acc_one<ENT>(acc, edge, k);
     Part mine = warp_part<ENT>(acc, k);
+    Row w{};            // warp 0: the row's sums
     float wide = 0.0f;  // M of a wide row in its second turn
     for (int turn = 0; turn < 2; turn++) {
         if (C > 1) {
@@ -651,10 +671,12 @@ __global__ void __launch_bounds__(NT * ROWS, 1024 / (NT * ROWS)) rows_kernel(con
             sync();
         }
         if (warp == 0) {
-            const Row w = turn ? join_wide(parts[1], C * NW, wide, k) : join_parts<ENT>(parts[0], C * NW, k);
-            Coef c = fill_coef(false);
-            if (turn || !w.wide) c = finish_row<ENT, POLICY>(a, r, w, in, rank == 0 && lane == 0);
-            if (lane == 0) coef = c, again = !turn && w.wide, wide_m = w.M;
+            w = turn ? join_wide(parts[1], C * NW, wide, k) : join_parts<ENT>(parts[0], C * NW, k);
+            if (POLICY && a.grad && (turn || !w.wide)) {
+                const Coef c = row_coef<ENT>(a, w, in);
+                if (lane == 0) coef = c;
+            }
+            if (lane == 0) again = !turn && w.wide, wide_m = w.M;
         }
         sync();
         if (!again) break;
@@ -662,6 +684,7 @@ __global__ void __launch_bounds__(NT * ROWS, 1024 / (NT * ROWS)) rows_kernel(con
         mine = wide_part<T, ENT>(row, a.V, wide, k, rank, C, tid, NT);
         sync();  // again and wide_m are written once more
     }
+    if (rank == 0 && tid == 0) write_row<ENT, POLICY>(a, r, w, in);
     launch_next();
     if (!POLICY || !a.grad) return;
 
@@ -932,10 +955,11 @@ __global__ void __launch_bounds__(Shape::NT + 64, Shape::CTAS) stream_kernel(con
                 w = join_wide(sh.wide_parts, C, w.M, k);
                 if (*abort) w.S = NAN;
             }
-            const Coef c = finish_row<ENT, true>(a, r, w, in, rank == 0 && lane == 0);
+            const Coef c = row_coef<ENT>(a, w, in);
             if (lane == 0) {
                 sh.coef[par] = c;
                 mbar_arrive(cbar_u + 8 * par);
+                if (rank == 0) write_row<ENT, true>(a, r, w, in);
             }
             __syncwarp();
         }
@@ -1092,10 +1116,10 @@ __global__ void __launch_bounds__(256, 6) grad_kernel(const Args a, const int pa
     const Slice s = slice_of(row, a.V, part, ROWS == 1 ? parts : 1, tid);
     Coef c = fill_coef(target >= a.V);
     if (target >= 0 && target < a.V) {
-        const float R = st.max * k;
+        const float R = rintf(st.max * k);
         const bool wide = fabsf(R) > WIDE && !isinf(st.max);
         // st.sum stands against M * k, the loop's terms against R
-        const float S = wide || isinf(st.max) ? st.sum : st.sum * ex2_approx(fmaf(st.max, k, -R));
+        const float S = wide || isinf(st.max) ? st.sum : st.sum * exp2f(fmaf(st.max, k, -R));
         c = make_coef(st.max, R, wide, S, ENT ? ent - logf(S) : 0.0f, g_lp, g_ent, (float)a.inv_t);
     }
     const int hot = target >= s.head ? (target - s.head) / N - s.lo : -1;

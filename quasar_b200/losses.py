@@ -18,7 +18,8 @@ from typing import NamedTuple, Optional
 from ._lib import BF16, F16, F32, check, lib
 
 _DTYPES = {}  # torch dtype -> the C constant; filled at the first call, torch being imported only then
-_raw = None   # the current stream's handle by device index, where torch has a way to it without a Stream object (2 us)
+# the current stream's handle by device index, where torch has a way to it without a Stream object (2 us)
+_raw = None
 
 
 class PolicyParams(ctypes.Structure):
@@ -131,8 +132,8 @@ def _p(t):
 
 
 def _on(torch, device, stream, tensors, call):
-    """call(the C stream) with the logits' device and the stream of the call current, so that what it allocates
-    belongs to that stream; keeps the call's tensors from being handed out again before the stream is done."""
+    """call(the C stream) with the logits' device and the stream of the call current, so that what it allocates belongs
+    to that stream; keeps the call's tensors from being handed out again before the stream is done."""
     if stream is None and torch.cuda.current_device() == device.index:
         return call(_raw(device.index) if _raw else torch.cuda.current_stream(device).cuda_stream)
     with torch.cuda.device(device):
@@ -250,15 +251,17 @@ def policy_loss(logits, targets, old_logprob, advantage, *, ref_logprob=None, we
         g = _like(torch, logits, rows, V, ld) if grad is True else buf
         if out is None:
             e = logits.new_empty
-            o = PolicyLoss(e((), dtype=f32), e(rows, dtype=f32), e(rows, dtype=f32) if want else None, e(rows, dtype=f32), g)
+            o = PolicyLoss(e((), dtype=f32), e(rows, dtype=f32), e(rows, dtype=f32) if want else None,
+                           e(rows, dtype=f32), g)
         else:
             o = PolicyLoss(out.loss, out.logprob, out.entropy, out.row_loss, g)
         check(lib().quasar_policy_loss(logits.data_ptr(), dt, ld, rows, V, targets.data_ptr(), old_logprob.data_ptr(),
-                                       advantage.data_ptr(), _p(ref_logprob), _p(weight), ctypes.addressof(prm), o.logprob.data_ptr(),
-                                       _p(o.entropy), o.row_loss.data_ptr(), o.loss.data_ptr(), _p(g),
-                                       0 if g is None else _ld(g), st), "quasar_policy_loss")
+                                       advantage.data_ptr(), _p(ref_logprob), _p(weight), ctypes.addressof(prm),
+                                       o.logprob.data_ptr(), _p(o.entropy), o.row_loss.data_ptr(), o.loss.data_ptr(),
+                                       _p(g), 0 if g is None else _ld(g), st), "quasar_policy_loss")
         return o
-    return _on(torch, device, stream, (logits, targets, old_logprob, advantage, ref_logprob, weight, buf, *(out or ())), call)
+    used = (logits, targets, old_logprob, advantage, ref_logprob, weight, buf, *(out or ()))
+    return _on(torch, device, stream, used, call)
 
 
 def preference_loss(logits, targets, cu_seqlens, *, ref_logprob=None, pair_weight=None, temperature: float = 1.0,
@@ -299,13 +302,15 @@ def preference_loss(logits, targets, cu_seqlens, *, ref_logprob=None, pair_weigh
                                e((rows, 2), dtype=f32), e(rows, dtype=f32), g)
         else:
             o = PreferenceLoss(*out[:6], g)
-        check(lib().quasar_preference_loss(logits.data_ptr(), dt, ld, rows, V, targets.data_ptr(), cu_seqlens.data_ptr(),
-                                           n // 2, _p(ref_logprob), _p(pair_weight), ctypes.addressof(prm), o.logprob.data_ptr(),
-                                           o.seq_logprob.data_ptr(), o.pair_loss.data_ptr(), o.loss.data_ptr(),
-                                           o.stats.data_ptr(), o.row_grad.data_ptr(), _p(g), 0 if g is None else _ld(g), st),
+        check(lib().quasar_preference_loss(logits.data_ptr(), dt, ld, rows, V, targets.data_ptr(),
+                                           cu_seqlens.data_ptr(), n // 2, _p(ref_logprob), _p(pair_weight),
+                                           ctypes.addressof(prm), o.logprob.data_ptr(), o.seq_logprob.data_ptr(),
+                                           o.pair_loss.data_ptr(), o.loss.data_ptr(), o.stats.data_ptr(),
+                                           o.row_grad.data_ptr(), _p(g), 0 if g is None else _ld(g), st),
               "quasar_preference_loss")
         return o
-    return _on(torch, device, stream, (logits, targets, cu_seqlens, ref_logprob, pair_weight, buf, *(out or ())), call)
+    used = (logits, targets, cu_seqlens, ref_logprob, pair_weight, buf, *(out or ()))
+    return _on(torch, device, stream, used, call)
 
 
 __all__ = ["TokenLogprobs", "PolicyLoss", "PreferenceLoss", "PolicyParams", "PreferenceParams", "token_logprobs",
