@@ -9,15 +9,14 @@
 // M is not known while the row streams, so a thread sums against a reference
 // that trails its running maximum and moves (one rescale of the sums) only
 // when a logit passes it by 2^LAG: terms stay below 2^LAG, far inside fp32,
-// and rescales are rare. A row whose M*k overflows (masked throughout by the
-// type's lowest value) is summed over again with t = (l - M) * k.
+// and rescales are rare. A row whose |M|*k passes 2^24 (masked throughout by a
+// large negative value) is summed over again with t = (l - M) * k.
 //
 // What bounds it: HBM for fp32 (4 bytes an element and pass); for 16-bit
 // types one exponential per element and pass on the special-function unit
 // (16 a clock and SM) takes 0.7 of the time that the bytes take.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
-#include <float.h>
 #include <math.h>
 
 #include <mutex>
@@ -32,8 +31,11 @@ namespace loss {
 constexpr int U = 4;           // 16-byte loads in flight per thread
 constexpr int MAXC = 8;        // CTAs of a row's cluster at most (the portable limit)
 constexpr float LAG = 20.0f;   // powers of two that a term may stand above the reference
-constexpr float WIDE = 1e37f;  // rows whose |M| * k passes this are summed with differences taken first
-constexpr float NEG = -FLT_MAX;
+// l * k - c is good to a fraction of 1 only while l * k is below 2^24 or so:
+// rows whose |M| * k reaches that are summed with differences taken first, and
+// no reference goes below it (masked logits of -1e9 or -1e30 end at 2^t = 0).
+constexpr float WIDE = 16777216.0f;
+constexpr float NEG = -WIDE;
 constexpr double LN2 = 0.6931471805599453094;
 
 template <typename T>
@@ -290,7 +292,7 @@ __device__ __forceinline__ Row join_parts(const Part* parts, int n, float k) {
     w.Q = ENT ? warp_sum((double)q) : 0.0;
     const float c = scaled(w.M, k);
     w.R = (double)c;
-    w.wide = fabsf(c) > WIDE && !isinf(w.M);
+    w.wide = !(fabsf(c) < WIDE) && !isinf(w.M);
     return w;
 }
 
@@ -536,7 +538,7 @@ __device__ __forceinline__ void remote_store(uint32_t addr, const Part& p) {
 
 // Sums of one thread's share of a slice against M itself, with differences
 // taken before the multiply: for rows whose maximum is so large, or so low,
-// that l * k overflows (a row masked throughout by the type's lowest value).
+// that l * k - R would keep nothing of t (a row masked throughout).
 template <typename T, bool ENT>
 __device__ __noinline__ Part wide_part(const T* row, int V, float M, float k, int part, int parts, int first, int nt) {
     const Slice sl = slice_of(row, V, part, parts, 0);
@@ -1117,7 +1119,7 @@ __global__ void __launch_bounds__(256, 6) grad_kernel(const Args a, const int pa
     Coef c = fill_coef(target >= a.V);
     if (target >= 0 && target < a.V) {
         const float R = rintf(st.max * k);
-        const bool wide = fabsf(R) > WIDE && !isinf(st.max);
+        const bool wide = !(fabsf(R) < WIDE) && !isinf(st.max);
         // st.sum stands against M * k, the loop's terms against R
         const float S = wide || isinf(st.max) ? st.sum : st.sum * exp2f(fmaf(st.max, k, -R));
         c = make_coef(st.max, R, wide, S, ENT ? ent - logf(S) : 0.0f, g_lp, g_ent, (float)a.inv_t);

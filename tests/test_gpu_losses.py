@@ -250,6 +250,39 @@ def test_rows_of_masks(dtype, V):
     assert (pol.grad[6:9] == 0).all() and (pol.logprob[6:9] == 0).all() and (pol.row_loss[6:9] == 0).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [1000, 40001])
+def test_rows_of_large_values(dtype, V):
+    """Masks of every size (-1e4 to -1e30) over parts of a row, over all of it, and large positive rows: the same
+    probabilities as with the row's maximum taken off first. t is formed from l - M, rounded like l itself."""
+    fills = [-1e4, -1e7, -1e9, -1e12, -1e20, -1e30, 1e6, 1e9, 1e20, 1e30]
+    rows = 4 * len(fills)
+    logits, targets, g = rows_of(rows, V, dtype, 19)
+    keep = torch.rand(V, generator=g, device="cuda") < 0.5
+    for i, f in enumerate(fills):
+        logits[4 * i] = f                                                      # the whole row
+        logits[4 * i + 1] = torch.where(keep, logits[4 * i + 1], torch.full_like(logits[0], f))  # half of it
+        logits[4 * i + 2, :V - 3] = f                                          # all but three
+        logits[4 * i + 3, V // 2] = f                                          # one
+        targets[4 * i + 1] = int(keep.nonzero()[7])
+        targets[4 * i + 2] = V - 2
+    lp, h = reference(logits, targets, 1.0)
+    out = q().token_logprobs(logits, targets, entropy=True)
+    close(out.logprob, lp, LP_ATOL + lp.abs() * 4 * EPS, "logprob")
+    close(out.entropy, h, H_ATOL, "entropy")
+    c, gh = torch.randn(rows, generator=g, device="cuda"), torch.randn(rows, generator=g, device="cuda")
+    ref, bound = reference_grad(logits, targets, 1.0, c, gh)
+    close(q().token_logprobs_grad(logits, targets, out.stats, c, entropy=out.entropy, grad_entropy=gh), ref, bound + 1e-30, "grad")
+    few = q().policy_loss(logits, targets, torch.full((rows,), -3.0, device="cuda"), c, entropy_coef=0.1)
+    many = [t.repeat(8, *[1] * (t.dim() - 1)) for t in (logits, targets, c)]   # 320 rows: the kernels of many rows
+    out = q().policy_loss(many[0], many[1], torch.full((8 * rows,), -3.0, device="cuda"), many[2], entropy_coef=0.1,
+                          weight=torch.full((8 * rows,), 1.0 / rows, device="cuda"))
+    fi = torch.finfo(dtype)
+    for j in range(0, 8 * rows, rows):
+        close(out.logprob[j:j + rows], few.logprob, 2 * LP_ATOL + lp.abs() * 8 * EPS)
+        close(out.grad[j:j + rows], few.grad, few.grad.double().abs() * (2 * fi.eps + 2e-4) + 1e-8)
+
+
 def policy64(lp, h, old, adv, ref, lo, hi, kl, ec):
     r = (lp - old.double()).exp()
     loss = -torch.minimum(r * adv.double(), r.clamp(1 - lo, 1 + hi) * adv.double())
