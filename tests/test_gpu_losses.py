@@ -461,6 +461,49 @@ def test_two_streamed_calls_at_once():
             assert all(torch.equal(x, y) for x, y in zip(a, b))
 
 
+def test_gradient_behind_copies_and_other_streams():
+    """The gradient's launch may start before the work in front of it has ended, and waits for it: behind a copy, a
+    fill, another stream's work, as the first of a graph and within one."""
+    rows, V = 64, 50021
+    logits, targets, g = rows_of(rows, V, torch.float32, 63)
+    c = torch.randn(rows, generator=g, device="cuda")
+    fwd = q().token_logprobs(logits, targets)
+    want = q().token_logprobs_grad(logits, targets, fwd.stats, c)
+    buf, derivative = torch.empty_like(logits), torch.empty_like(c)
+    side = torch.cuda.Stream()
+
+    def work():
+        buf.zero_()
+        derivative.zero_()
+        a = q().token_logprobs_grad(buf, targets, fwd.stats, derivative)       # zeros
+        here = torch.cuda.current_stream()
+        side.wait_stream(here)
+        with torch.cuda.stream(side):
+            buf.copy_(logits)
+            derivative.copy_(c)
+        here.wait_stream(side)
+        b = q().token_logprobs_grad(buf, targets, fwd.stats, derivative)
+        q().token_logprobs_grad(buf, targets, fwd.stats, derivative, out=buf)  # in place, behind its own reading
+        d = buf.clone()
+        buf.fill_(7.0)
+        return a, b, d
+
+    def check(res):
+        torch.cuda.synchronize()
+        assert (res[0] == 0).all() and torch.equal(res[1], want) and torch.equal(res[2], want)
+
+    for _ in range(5):
+        check(work())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        first = q().token_logprobs_grad(logits, targets, fwd.stats, c)
+        res = work()
+    for _ in range(5):
+        graph.replay()
+        check(res)
+        assert torch.equal(first, want)
+
+
 def test_first_calls_under_capture():
     """A process whose first calls are captured, without a call before that sets the kernels up."""
     code = """
