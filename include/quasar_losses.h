@@ -143,7 +143,8 @@ typedef struct {
  *                   rows get no gradient.
  *   d_ref_logprob   [2*pairs] the reference model's scores (sums, or means
  *                   with length_normalize), or NULL for 0.
- *   d_pair_weight   [pairs], or NULL for 1/pairs each.
+ *   d_pair_weight   [pairs], or NULL for 1/pairs each. A pair of weight 0
+ *                   takes no part in loss and gradient.
  *   d_logprob       [rows] out, per token.
  *   d_seq_logprob   [2*pairs] out: the sums over the sequences.
  *   d_pair_loss     [pairs] out;  d_loss [1] out.

@@ -140,7 +140,7 @@ int quasar_preference_loss(const void* d_logits, int dtype, int64_t ld, int rows
         a.row_grad = d_row_grad;
         rc = status(qs::loss::launch_rows(a, dtype, st));
     }
-    if (rc == QUASAR_OK && pairs > 0) {
+    if (rc == QUASAR_OK) {
         qs::loss::PairArgs p;
         memset(&p, 0, sizeof p);
         p.logprob = d_logprob;
@@ -157,9 +157,8 @@ int quasar_preference_loss(const void* d_logits, int dtype, int64_t ld, int rows
         p.seq = d_seq_logprob;
         p.pair_loss = d_pair_loss;
         p.row_grad = d_row_grad;
-        rc = status(qs::loss::launch_pairs(p, st));
+        rc = status(qs::loss::launch_pairs(p, d_loss, st));
     }
-    if (rc == QUASAR_OK) rc = status(qs::loss::launch_weighted_sum(d_pair_loss, d_pair_weight, pairs, d_loss, st));
     if (rc == QUASAR_OK && rows > 0 && d_grad) {
         a.stats_in = d_stats;
         a.g_lp = d_row_grad;

@@ -1167,22 +1167,23 @@ __device__ __forceinline__ double cta_sum(double x, double* buf, int threads) {
     return s;
 }
 
-// One CTA per pair.
-__global__ void __launch_bounds__(128) pair_kernel(const PairArgs p) {
-    __shared__ double buf[4];
-    wait_before();
-    launch_next();
-    const int i = blockIdx.x, tid = threadIdx.x;
+__device__ __forceinline__ double pair_weight(const PairArgs& p, int i) { return p.weight ? (double)p.weight[i] : 1.0 / p.pairs; }
+
+// Pair i by a warp, or by the CTA's 128 threads: its outputs and its rows'
+// derivatives. Returns its loss in 64 bits.
+template <bool WARP>
+__device__ __forceinline__ double pair_loss(const PairArgs& p, int i, int tid, double* buf) {
+    constexpr int NT = WARP ? 32 : 128;
     const int at[3] = {p.cu[2 * i], p.cu[2 * i + 1], p.cu[2 * i + 2]};
     const bool ok = at[0] >= 0 && at[0] <= at[1] && at[1] <= at[2] && at[2] <= p.rows;
     double sum[2] = {0.0, 0.0}, n[2] = {0.0, 0.0};
     if (ok) {
         for (int s = 0; s < 2; s++) {
             double x = 0.0, c = 0.0;
-            for (int64_t r = at[s] + tid; r < at[s + 1]; r += 128)
+            for (int64_t r = at[s] + tid; r < at[s + 1]; r += NT)
                 if (p.targets[r] >= 0) x += (double)p.logprob[r], c += 1.0;
-            sum[s] = cta_sum(x, buf, 128);
-            n[s] = cta_sum(c, buf, 128);
+            sum[s] = WARP ? warp_sum(x) : cta_sum(x, buf, NT);
+            n[s] = WARP ? warp_sum(c) : cta_sum(c, buf, NT);
         }
     } else {
         sum[0] = sum[1] = NAN;
@@ -1198,18 +1199,47 @@ __global__ void __launch_bounds__(128) pair_kernel(const PairArgs p) {
     const double up = fmax(-x, 0.0) + tail, down = fmax(x, 0.0) + tail;
     const double sn = 1.0 / (1.0 + exp(x)), sp = 1.0 / (1.0 + exp(-x));
     // a share of 0 takes nothing, of an infinite loss either
-    const double loss = (p.eps != 1.0 ? (1.0 - p.eps) * up : 0.0) + (p.eps != 0.0 ? p.eps * down : 0.0);
-    const double w = p.weight ? (double)p.weight[i] : 1.0 / p.pairs;
-    const double g = -p.beta * ((1.0 - p.eps) * sn - p.eps * sp) * w * p.scale;
+    const double loss = x != x ? NAN : (p.eps != 1.0 ? (1.0 - p.eps) * up : 0.0) + (p.eps != 0.0 ? p.eps * down : 0.0);
+    const double w = pair_weight(p, i);
+    const double g = w != 0.0 ? -p.beta * ((1.0 - p.eps) * sn - p.eps * sp) * w * p.scale : 0.0;
     if (tid == 0) {
         p.seq[2 * i] = (float)sum[0];
         p.seq[2 * i + 1] = (float)sum[1];
-        p.pair_loss[i] = (float)(x == x ? loss : NAN);
+        p.pair_loss[i] = (float)loss;
     }
     if (ok)
         for (int s = 0; s < 2; s++)
-            for (int64_t r = at[s] + tid; r < at[s + 1]; r += 128)
+            for (int64_t r = at[s] + tid; r < at[s + 1]; r += NT)
                 if (p.targets[r] >= 0) p.row_grad[r] = (float)((s ? -g : g) * by[s]);
+    return loss;
+}
+
+// One CTA per pair.
+__global__ void __launch_bounds__(128) pair_kernel(const PairArgs p) {
+    __shared__ double buf[4];
+    wait_before();
+    launch_next();
+    pair_loss<false>(p, (int)blockIdx.x, (int)threadIdx.x, buf);
+}
+
+// A warp per pair, and their weighted sum: for the pairs of a small batch,
+// where a launch weighs more than the longer loops.
+constexpr int FEW_PAIRS = 16, FEW_ROWS = 512;
+__global__ void __launch_bounds__(32 * FEW_PAIRS) few_pairs_kernel(const PairArgs p, float* out) {
+    __shared__ double part[FEW_PAIRS];
+    wait_before();
+    launch_next();
+    const int i = (int)threadIdx.x / 32;
+    if (i < p.pairs) {
+        const double loss = pair_loss<true>(p, i, (int)threadIdx.x % 32, nullptr), w = pair_weight(p, i);
+        if (threadIdx.x % 32 == 0) part[i] = w != 0.0 ? w * loss : 0.0;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        double s = 0.0;
+        for (int j = 0; j < p.pairs; j++) s += part[j];
+        out[0] = (float)s;
+    }
 }
 
 // One CTA: the same order of sums in every run. A weight of 0 takes nothing,
@@ -1403,7 +1433,14 @@ cudaError_t launch_grad(const Args& a, int dtype, cudaStream_t st) {
     return grad_typed<__nv_bfloat16>(a, st);
 }
 
-cudaError_t launch_pairs(const PairArgs& p, cudaStream_t st) { return launch(pair_kernel, (unsigned)p.pairs, 128, 0, 0, true, st, p); }
+cudaError_t launch_pairs(const PairArgs& p, float* loss, cudaStream_t st) {
+    if (p.pairs > 0 && p.pairs <= FEW_PAIRS && p.rows <= FEW_ROWS) return launch(few_pairs_kernel, 1u, 32 * FEW_PAIRS, 0, 0, true, st, p, loss);
+    if (p.pairs > 0) {
+        const cudaError_t e = launch(pair_kernel, (unsigned)p.pairs, 128, 0, 0, true, st, p);
+        if (e != cudaSuccess) return e;
+    }
+    return launch_weighted_sum(p.pair_loss, p.weight, p.pairs, loss, st);
+}
 
 cudaError_t launch_weighted_sum(const float* x, const float* w, int n, float* out, cudaStream_t st) {
     return launch(weighted_sum_kernel, 1u, 1024, 0, 0, true, st, x, w, n, out);

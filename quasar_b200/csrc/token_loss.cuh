@@ -60,8 +60,8 @@ struct PairArgs {
 cudaError_t launch_rows(const Args& a, int dtype, cudaStream_t st);
 // The gradient into the logits from given per-row derivatives.
 cudaError_t launch_grad(const Args& a, int dtype, cudaStream_t st);
-// Sequence sums, pair losses and the rows' derivatives.
-cudaError_t launch_pairs(const PairArgs& p, cudaStream_t st);
+// Sequence sums, pair losses, their weighted sum and the rows' derivatives.
+cudaError_t launch_pairs(const PairArgs& p, float* loss, cudaStream_t st);
 // out[0] = sum of w[i] * x[i] (w NULL: 1/n each), in index order by blocks.
 cudaError_t launch_weighted_sum(const float* x, const float* w, int n, float* out, cudaStream_t st);
 

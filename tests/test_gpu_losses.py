@@ -619,6 +619,21 @@ def test_infinite_preferences():
     assert out.loss.item() == 0 and (out.grad == 0).all()
 
 
+def test_pairs_of_weight_zero():
+    """A pair of weight 0 takes no part: no gradient, and nothing of its loss, NaN among it."""
+    for n in (2, 20):                                   # few pairs and more
+        logits, targets, g = rows_of(4 * n, 50, torch.float32, 34)
+        logits[5] = math.nan
+        cu = torch.arange(0, 4 * n + 1, 2, dtype=torch.int32, device="cuda")
+        w = torch.ones(n, device="cuda")
+        w[1] = 0
+        out = q().preference_loss(logits, targets, cu, pair_weight=w)
+        assert torch.isfinite(out.loss) and torch.isnan(out.pair_loss[1]) and (out.grad[4:8] == 0).all()
+        assert torch.isfinite(out.grad).all()
+        rest = torch.arange(n, device="cuda") != 1
+        close(out.loss, out.pair_loss[rest].double().sum(), 4 * n * EPS)
+
+
 def test_preference_offsets_that_leave_the_rows():
     """Offsets that fall or leave the rows: NaN for the pair and the loss, no gradient for its rows, the other pairs as ever."""
     logits, targets, g = rows_of(12, 77, torch.float32, 32)
