@@ -20,6 +20,7 @@
 #include <math.h>
 
 #include <mutex>
+#include <type_traits>
 
 #include "common.cuh"
 #include "ptx.cuh"
@@ -1322,9 +1323,16 @@ static cudaError_t rows_by_size(const Args& a, cudaStream_t st) {
     return rows_launch<T, ENT, POLICY, 256, 1>(a, C, st);
 }
 
-// Long rows: one CTA of 640 consumers per SM with chunks of 30 KB. Middle
-// ones, of which an SM can hold two, two CTAs of 256 with chunks of 20 KB.
-using StreamLong = StreamShape<640, 1, 3, 7>;
+// Long rows: one CTA of 640 consumers per SM with chunks of 30 KB, and of 448
+// with chunks of 28 KB for the entropy of 16-bit types, which is bound by
+// instructions and gains from 119 registers a thread instead of 80 (bf16,
+// V = 151936, 2000 rows 256 us against 276, 1023 rows 116 and 123; V = 200000,
+// 1500 rows 236 and 265). Without entropy 640 are faster (V = 200000, 220 and
+// 227), and in fp32, bound by memory (2000 rows with entropy 399 and 418).
+// Middle rows, of which an SM can hold two: two CTAs of 256 with chunks of 20 KB.
+template <typename T, bool ENT>
+using StreamLong =
+    std::conditional_t<ENT && sizeof(T) == 2, StreamShape<448, 1, 4, 7>, StreamShape<640, 1, 3, 7>>;
 using StreamMiddle = StreamShape<256, 2, 5, 5>;
 static constexpr int64_t STREAM_MIN = 96 * 1024, STREAM_MIDDLE = 128 * 1024, STREAM_L2 = 32 << 20;
 
@@ -1391,7 +1399,7 @@ static cudaError_t policy_by_size(const Args& a, cudaStream_t st) {
     if (row_bytes > STREAM_MIDDLE && a.rows >= SMS) {
         int C = 1;
         while (C < MAXC && SMS / C * row_bytes > STREAM_L2) C *= 2;
-        return stream_launch<T, ENT, StreamLong>(a, C, st);
+        return stream_launch<T, ENT, StreamLong<T, ENT>>(a, C, st);
     }
     return rows_by_size<T, ENT, true>(a, st);
 }
