@@ -12,6 +12,7 @@
  * after the launch. No call allocates, synchronises or keeps anything between
  * calls: every buffer, scratch included, is the caller's, so calls that use
  * different buffers may overlap and every call can be captured into a graph.
+ * Outputs are apart from inputs and from each other but where it says may be.
  * Results do not depend on the run: no sum is formed by atomics.
  *
  * Rows. Row r of `rows` holds V logits at d_logits + r*ld (elements of dtype,
@@ -103,7 +104,7 @@ typedef struct {
  *   d_ref_logprob   [rows], or NULL with kl_coef == 0.
  *   d_weight        [rows], or NULL for 1/rows each. A row of weight 0 takes
  *                   no part, like one with a negative target.
- *   d_logprob       [rows] out.
+ *   d_logprob       [rows] out; may be d_old_logprob or d_ref_logprob.
  *   d_entropy       [rows] out, or NULL.
  *   d_row_loss      [rows] out (not multiplied by the weight).
  *   d_loss          [1] out.
@@ -146,7 +147,8 @@ typedef struct {
  *   d_pair_weight   [pairs], or NULL for 1/pairs each. A pair of weight 0
  *                   takes no part in loss and gradient.
  *   d_logprob       [rows] out, per token.
- *   d_seq_logprob   [2*pairs] out: the sums over the sequences.
+ *   d_seq_logprob   [2*pairs] out: the sums over the sequences; may be
+ *                   d_ref_logprob.
  *   d_pair_loss     [pairs] out;  d_loss [1] out.
  *   d_stats         [rows] out;  d_row_grad [rows] out: the derivative of the
  *                   loss by each token's log-probability, times grad_scale.

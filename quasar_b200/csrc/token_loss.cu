@@ -1177,6 +1177,8 @@ __device__ __forceinline__ double pair_loss(const PairArgs& p, int i, int tid, d
     constexpr int NT = WARP ? 32 : 128;
     const int at[3] = {p.cu[2 * i], p.cu[2 * i + 1], p.cu[2 * i + 2]};
     const bool ok = at[0] >= 0 && at[0] <= at[1] && at[1] <= at[2] && at[2] <= p.rows;
+    // before the sums, whose barriers stand between these and the outputs: seq may be ref
+    const double ref[2] = {p.ref ? (double)p.ref[2 * i] : 0.0, p.ref ? (double)p.ref[2 * i + 1] : 0.0};
     double sum[2] = {0.0, 0.0}, n[2] = {0.0, 0.0};
     if (ok) {
         for (int s = 0; s < 2; s++) {
@@ -1192,7 +1194,7 @@ __device__ __forceinline__ double pair_loss(const PairArgs& p, int i, int tid, d
     double score[2], by[2];
     for (int s = 0; s < 2; s++) {
         by[s] = p.mean && n[s] > 0.0 ? 1.0 / n[s] : 1.0;
-        score[s] = sum[s] * by[s] - (p.ref ? (double)p.ref[2 * i + s] : 0.0);
+        score[s] = sum[s] * by[s] - ref[s];
     }
     const double x = p.beta * (score[0] - score[1]);
     // softplus(-x) and softplus(x); sigmoid(-x) and sigmoid(x)

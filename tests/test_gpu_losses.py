@@ -692,6 +692,36 @@ def test_out_is_written_again():
         q().token_logprobs(logits, targets, out=out)
 
 
+@pytest.mark.parametrize("shape", [(3, 97), (6, 60000), (40, 9001), (700, 60001), (200, 151936)])
+def test_inputs_from_the_buffers_of_out(shape):
+    """Log-probabilities of an earlier call as the old (or reference) ones, whose tensors the call writes again."""
+    rows, V = shape
+    logits, targets, g = rows_of(rows, V, torch.bfloat16, 18)
+    targets[rows // 2] = -1
+    adv = torch.randn(rows, generator=g, device="cuda")
+    first = q().policy_loss(logits, targets, torch.zeros(rows, device="cuda"), adv)
+    old = first.logprob + 0.1 * torch.randn(rows, generator=g, device="cuda")
+    want = q().policy_loss(logits, targets, old, adv, ref_logprob=old, kl_coef=0.5)
+    for _ in range(3):
+        first.logprob.copy_(old)
+        got = q().policy_loss(logits, targets, first.logprob, adv, ref_logprob=first.logprob, kl_coef=0.5, out=first)
+        assert got.logprob is first.logprob
+        assert all(torch.equal(a, b) for a, b in zip(got, want) if a is not None)
+
+
+@pytest.mark.parametrize("pairs,length", [(3, 5), (40, 3), (2, 400)])
+def test_reference_scores_from_the_buffers_of_out(pairs, length):
+    logits, targets, g = rows_of(2 * pairs * length, 97, torch.float32, 19)
+    cu = torch.arange(0, 2 * pairs * length + 1, length, dtype=torch.int32, device="cuda")
+    first = q().preference_loss(logits, targets, cu, grad=False)
+    ref = first.seq_logprob + torch.randn(2 * pairs, generator=g, device="cuda")
+    want = q().preference_loss(logits, targets, cu, ref_logprob=ref)
+    for _ in range(20):
+        first.seq_logprob.copy_(ref)
+        got = q().preference_loss(logits, targets, cu, ref_logprob=first.seq_logprob, out=first)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_refusals():
     logits, targets, g = rows_of(4, 64, torch.float32, 17)
     f = torch.zeros(4, device="cuda")
