@@ -34,7 +34,9 @@
  * log-probabilities, entropies and losses are formed in 64 bits from them and
  * rounded once; gradients are formed in 32 bits and rounded once to dtype. A row whose derivatives by
  * log-probability and entropy are both 0 (a clipped ratio) has a gradient of
- * zeros, whatever its logits. */
+ * zeros, whatever its logits. A derivative that is infinite or passes the fp32
+ * range gives infinities with their signs where p is not 0, and zeros where it
+ * is. */
 #ifndef QUASAR_LOSSES_H
 #define QUASAR_LOSSES_H
 
@@ -99,7 +101,9 @@ typedef struct {
  *   loss     = sum_r weight_r * row_loss_r
  * The gradient takes ratio, KL term and entropy as functions of the logits
  * (old and ref log-probabilities, advantages and weights are constants); a
- * ratio at a border counts as not clipped.
+ * ratio at a border counts as not clipped, and an advantage of 0 takes nothing
+ * of a ratio, an infinite one either. Ratio and KL factor may pass the fp32
+ * range as long as their products with weight and grad_scale do not.
  *   d_old_logprob, d_advantage   [rows].
  *   d_ref_logprob   [rows], or NULL with kl_coef == 0.
  *   d_weight        [rows], or NULL for 1/rows each. A row of weight 0 takes

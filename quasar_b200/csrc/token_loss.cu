@@ -305,7 +305,11 @@ struct Coef {
     float lt;  // the target's logit
     int kind;  // ROW_*
 };
-enum { ROW_SUM = 0, ROW_ZERO = 1, ROW_NAN = 2, ROW_WIDE = 3 };  // ROW_WIDE: c is M itself, t = (l - c) * k
+// ROW_WIDE: c is M itself, t = (l - c) * k; ROW_STEEP: a or b is infinite. The
+// first three take their elements one by one.
+enum { ROW_SUM = 0, ROW_WIDE = 1, ROW_STEEP = 2, ROW_ZERO = 3, ROW_NAN = 4 };
+
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.402823466e38f; }
 
 // The gradient of g_lp * logprob + g_ent * entropy: p_v = 2^t / S and
 // ln p_v = ln2 * t - ln S, so (g_lp ([v==target] - p) - g_ent p (ln p + H)) / T
@@ -319,7 +323,16 @@ __device__ __forceinline__ Coef make_coef(float M, float R, bool wide, float S, 
     o.b = w * (float)LN2 * g_ent;
     o.one = g_lp * inv_t;
     o.lt = 0.0f;
-    o.kind = (g_lp == 0.0f && g_ent == 0.0f) ? ROW_ZERO : S != S ? ROW_NAN : M == -INFINITY ? ROW_ZERO : wide ? ROW_WIDE : ROW_SUM;
+    if (g_lp == 0.0f && g_ent == 0.0f)
+        o.kind = ROW_ZERO;
+    else if (S != S)
+        o.kind = ROW_NAN;
+    else if (M == -INFINITY)
+        o.kind = ROW_ZERO;
+    else if (o.a != o.a || o.b != o.b)
+        o.kind = ROW_NAN;
+    else
+        o.kind = wide ? ROW_WIDE : finite(o.a) && finite(o.b) ? ROW_SUM : ROW_STEEP;
     return o;
 }
 // A row without an element-wise gradient.
@@ -355,26 +368,38 @@ __device__ __forceinline__ double row_logprob(const Args& a, const Row& w, float
 }
 
 // The policy loss's derivative by the row's log-probability. F: the precision;
-// a ratio at a border counts as not clipped.
+// a ratio at a border counts as not clipped, and an advantage of 0 takes
+// nothing of an infinite ratio.
 template <typename F>
-__device__ __forceinline__ F policy_slope(const Args& a, F adv, F ratio, F eu, F* loss) {
-    const F lo = (F)(1.0 - a.clip_lo), hi = (F)(1.0 + a.clip_hi);
+__device__ __forceinline__ F policy_slope(F lo, F hi, F kl, F adv, F ratio, F eu, F* loss) {
+    if (adv == (F)0 && ratio == ratio) ratio = (F)1;
     const F fit = ratio < lo ? lo : ratio > hi ? hi : ratio;  // NaN stays
     const F x = ratio * adv, y = fit * adv;
     *loss = x <= y ? -x : y < x ? -y : (F)NAN;
-    return (x <= y ? -x : y < x ? (F)0 : (F)NAN) - (a.kl != 0.0 ? (F)a.kl * eu : (F)0);
+    return (x <= y ? -x : y < x ? (F)0 : (F)NAN) - (kl != (F)0 ? kl * eu : (F)0);
+}
+
+// The same in 64 bits, times the row's weight: for rows whose ratio or KL
+// factor passes fp32 (differences of log-probabilities above 88), where slope
+// times weight may still fit.
+__device__ __noinline__ float steep_slope(double lo, double hi, double kl, float adv, double d, double u, double ws) {
+    double loss;
+    return (float)(policy_slope<double>(lo, hi, kl, adv, exp(d), expm1(u), &loss) * ws);
 }
 
 // A row's gradient coefficients. All the row's threads wait for them, so the
 // exponentials of differences of log-probabilities, which are near 1, are
-// expf's here (2^-23 relative); their 64-bit forms took 1.4 us.
+// expf's here (2^-23 relative); their 64-bit forms took 1.4 us, and are taken
+// where 32 bits overflow.
 template <bool ENT>
 __device__ __forceinline__ Coef row_coef(const Args& a, const Row& w, const RowIn& in) {
     const double lp = row_logprob(a, w, in.lt);
-    const float S = (float)w.S, ratio = expf((float)(lp - (double)in.old_lp));
-    const float eu = a.kl != 0.0 ? expm1f((float)((double)in.ref_lp - lp)) : 0.0f;
+    const double d = lp - (double)in.old_lp, u = a.kl != 0.0 ? (double)in.ref_lp - lp : 0.0;
+    const float S = (float)w.S, ratio = expf((float)d), eu = a.kl != 0.0 ? expm1f((float)u) : 0.0f;
     float loss;
-    const float ws = (float)(in.weight * a.scale), g = policy_slope<float>(a, in.adv, ratio, eu, &loss) * ws;
+    const float ws = (float)(in.weight * a.scale);
+    float g = policy_slope<float>((float)(1.0 - a.clip_lo), (float)(1.0 + a.clip_hi), (float)a.kl, in.adv, ratio, eu, &loss) * ws;
+    if (!finite(g)) g = steep_slope(1.0 - a.clip_lo, 1.0 + a.clip_hi, a.kl, in.adv, d, u, in.weight * a.scale);
     Coef c = make_coef(w.M, (float)w.R, w.wide, S, ENT ? (float)-LN2 * ((float)w.Q / S) : 0.0f, g, ENT ? -(float)a.ec * ws : 0.0f, (float)a.inv_t);
     c.lt = in.lt;
     return c;
@@ -400,7 +425,7 @@ __device__ __forceinline__ void write_row(const Args& a, int64_t r, const Row& w
     if (POLICY) {
         const double u = a.kl != 0.0 ? (double)in.ref_lp - lp : 0.0, eu = a.kl != 0.0 ? expm1(u) : 0.0;
         double loss;
-        policy_slope<double>(a, in.adv, exp(lp - (double)in.old_lp), eu, &loss);
+        policy_slope<double>(1.0 - a.clip_lo, 1.0 + a.clip_hi, a.kl, in.adv, exp(lp - (double)in.old_lp), eu, &loss);
         if (a.kl != 0.0) loss += a.kl * (isinf(eu) ? eu : eu - u);
         if (ENT && a.ec != 0.0) loss -= a.ec * H;
         a.row_loss[r] = (float)loss;
@@ -422,8 +447,14 @@ __device__ __forceinline__ void blank_row(const Args& a, int64_t r, float v) {
 template <bool ENT>
 __device__ __forceinline__ float grad1(const Coef& c, float l, float k) {
     const float t = c.kind == ROW_WIDE ? (l - c.c) * k : fmaf(l, k, -c.c);
-    const float e = ex2_approx(t);
-    return ENT ? e * fmaf(c.b, fmaxf(t, -200.0f), c.a) : e * c.a;
+    const float e = ex2_approx(t), f = ENT ? fmaf(c.b, fmaxf(t, -200.0f), c.a) : c.a;
+    return e == 0.0f && !finite(f) ? 0.0f : e * f;
+}
+
+// The target's: an infinite derivative stays what it is.
+template <bool ENT>
+__device__ __forceinline__ float grad_target(const Coef& c, float l, float k) {
+    return finite(c.one) ? grad1<ENT>(c, l, k) + c.one : c.one;
 }
 
 // A pack's gradient (rows of ROW_SUM).
@@ -449,9 +480,9 @@ __device__ __forceinline__ uint4 grad_of(const uint4& p, const Coef& c, float k)
     return narrow(x, (T*)nullptr);
 }
 
-// The same for rows of ROW_WIDE (rare: out of the streaming loops).
+// The same for rows of the other kinds (rare: out of the streaming loops).
 template <typename T, bool ENT>
-__device__ __noinline__ uint4 grad_of_wide(uint4 p, Coef c, float k) {
+__device__ __noinline__ uint4 grad_of_rare(uint4 p, Coef c, float k) {
     float x[Type<T>::N];
     widen(p, x, (T*)nullptr);
 #pragma unroll
@@ -459,7 +490,7 @@ __device__ __noinline__ uint4 grad_of_wide(uint4 p, Coef c, float k) {
     return narrow(x, (T*)nullptr);
 }
 
-__device__ __forceinline__ bool elementwise(const Coef& c) { return c.kind == ROW_SUM || c.kind == ROW_WIDE; }
+__device__ __forceinline__ bool elementwise(const Coef& c) { return c.kind <= ROW_STEEP; }
 
 // A pack of zeros, or of NaN.
 template <typename T>
@@ -488,11 +519,11 @@ __device__ __noinline__ void store_elements(T* dst, uint4 p) {
 // An edge element's gradient.
 template <typename T, bool ENT>
 __device__ __forceinline__ void put_edge(T* out, int v, int target, float l, const Coef& c, float k) {
-    put1(out + v, c.kind == ROW_ZERO ? 0.0f : c.kind == ROW_NAN ? NAN : grad1<ENT>(c, l, k) + (v == target ? c.one : 0.0f));
+    put1(out + v, c.kind == ROW_ZERO ? 0.0f : c.kind == ROW_NAN ? NAN : v == target ? grad_target<ENT>(c, l, k) : grad1<ENT>(c, l, k));
 }
 
 // Writes a row's gradient where no batch loop fits: element-wise gradients of
-// wide rows, fills, and rows of another 16-byte phase than the logits'.
+// rows of the rare kinds, fills, and rows of another 16-byte phase than the logits'.
 // Packs [lo, hi), pack lo + i by thread i % nt.
 template <typename T, bool ENT>
 __device__ __noinline__ void grad_plain(const T* row, T* out, int head, int lo, int hi, Coef c, float k, int tid, int nt) {
@@ -505,7 +536,7 @@ __device__ __noinline__ void grad_plain(const T* row, T* out, int head, int lo, 
         uint4 g = fill;
         if (elementwise(c)) {
             const uint4 p = load_pack(src + v);
-            g = c.kind == ROW_SUM ? grad_of<T, ENT>(p, c, k) : grad_of_wide<T, ENT>(p, c, k);
+            g = c.kind == ROW_SUM ? grad_of<T, ENT>(p, c, k) : grad_of_rare<T, ENT>(p, c, k);
         }
         if (same)
             reinterpret_cast<uint4*>(dst)[v] = g;
@@ -721,7 +752,7 @@ __global__ void __launch_bounds__(NT * ROWS, 1024 / (NT * ROWS)) rows_kernel(con
         grad_plain<T, ENT>(row, out, s.head, s.lo, s.lo + s.n, c, k, tid, NT);
     }
     // the thread that wrote the target's pack puts the target right
-    if (hot >= 0 && hot < s.n && tid == hot_thread && elementwise(c)) put1(out + target, grad1<ENT>(c, c.lt, k) + c.one);
+    if (hot >= 0 && hot < s.n && tid == hot_thread && elementwise(c)) put1(out + target, grad_target<ENT>(c, c.lt, k));
 }
 
 // ---- a stream of rows per cluster ----------------------------------------------
@@ -1049,7 +1080,7 @@ __global__ void __launch_bounds__(Shape::NT + 64, Shape::CTAS) stream_kernel(con
                         for (int u = 0; u < PP; u++)
                             if (base + u * NT < b.n) {
                                 const uint4 p = lds_pack(at + u * NT * 16);
-                                const uint4 g = c.kind == ROW_SUM ? grad_of<T, ENT>(p, c, k) : c.kind == ROW_WIDE ? grad_of_wide<T, ENT>(p, c, k) : fill_pack<T>(c);
+                                const uint4 g = c.kind == ROW_SUM ? grad_of<T, ENT>(p, c, k) : elementwise(c) ? grad_of_rare<T, ENT>(p, c, k) : fill_pack<T>(c);
                                 if (same)
                                     __stcs(d + u * NT, g);
                                 else
@@ -1066,7 +1097,7 @@ __global__ void __launch_bounds__(Shape::NT + 64, Shape::CTAS) stream_kernel(con
                 if (b.edge >= 0) put_edge<T, ENT>(b_out, b.edge, b_target, b_edge, c, k);
                 // the thread that wrote the target's pack puts the target right
                 const int hot = b_target >= b.head ? (b_target - b.head) / N - b.lo : -1;
-                if (hot >= 0 && hot < b.n && hot % NT == tid && elementwise(c)) put1(b_out + b_target, grad1<ENT>(c, c.lt, k) + c.one);
+                if (hot >= 0 && hot < b.n && hot % NT == tid && elementwise(c)) put1(b_out + b_target, grad_target<ENT>(c, c.lt, k));
             }
             if (more) {
                 b_out = (T*)a.grad + r * a.grad_ld;
@@ -1152,7 +1183,7 @@ __global__ void __launch_bounds__(256, 6) grad_kernel(const Args a, const int pa
     } else {
         grad_plain<T, ENT>(row, out, s.head, s.lo, s.lo + s.n, c, k, tid, NT);
     }
-    if (mine) put1(out + target, grad1<ENT>(c, lt, k) + c.one);
+    if (mine) put1(out + target, grad_target<ENT>(c, lt, k));
 }
 
 // ---- pairs and sums --------------------------------------------------------------

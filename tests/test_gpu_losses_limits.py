@@ -1,0 +1,107 @@
+"""Token log-probabilities and losses at the ends of their ranges: ratios and derivatives beyond fp32, targets and
+offsets out of range, waits that run out, sizes beyond 32 bits, and the accuracy of entropies. Plain 64-bit
+implementations and bounds are those of test_gpu_losses.py."""
+import ctypes
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from tests.test_gpu_losses import DTYPES, EPS, H_ATOL, LP_ATOL, close, q, reference, reference_grad, rows_of, softmax64  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+
+# a warp per row, clusters, and the streaming kernel for rows of 100 to 128 KB and for longer ones
+RANGES = [(40, 1000), (12, 50021), (600, 30001), (160, 75001)]
+
+
+def banned_rows(rows, V, dtype, seed):
+    """Rows with a third of the columns banned, other than the targets'."""
+    logits, targets, g = rows_of(rows, V, dtype, seed)
+    ban = torch.rand(V, generator=g, device="cuda") < 1 / 3
+    at = targets.long()[:, None]
+    keep = logits.gather(1, at)
+    logits.masked_fill_(ban, -math.inf)
+    logits.scatter_(1, at, keep)
+    return logits, targets, g
+
+
+@pytest.mark.parametrize("entropy_coef", [0.0, 0.01])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", RANGES, ids=str)
+def test_ratios_beyond_fp32(shape, dtype, entropy_coef):
+    """Ratios that fp32 does not hold: an advantage of 0 takes no part whatever the ratio, a positive one is clipped,
+    and a negative one's slope counts with its weight. The log-probability's error goes into ratio and slope as in
+    test_policy_loss."""
+    rows, V = shape
+    logits, targets, g = banned_rows(rows, V, dtype, 80)
+    lp, h = reference(logits, targets, 1.0)
+    kind = torch.arange(rows, device="cuda") % 8
+    far = torch.tensor([110.0, 800.0, math.inf, 110.0, 91.0, 0.5, -110.0, 91.0], device="cuda", dtype=torch.float64)
+    adv = torch.tensor([0.0, 0.0, 0.0, 1.0, -1.0, -2.0, 0.0, 0.5], device="cuda")[kind]
+    old = (lp - far[kind]).float()
+    steep = kind == 4
+    weight = torch.where(steep, 1e-37, 1.0 / rows).float()
+    for kl in (0.0, 0.05):
+        # the KL term's exponential beyond fp32, in rows of small weight
+        ref = (lp + torch.where(steep | (kind == 7), 91.0 if kl else 0.0, 0.3)).float()
+        w = torch.where(kind == 7, 1e-37, weight).float() if kl else weight
+        kw = dict(ref_logprob=ref, kl_coef=kl, entropy_coef=entropy_coef)
+        out = q().policy_loss(logits, targets, old, adv, weight=w, **kw)
+        r, u, a = (lp - old.double()).exp(), ref.double() - lp, adv.double()
+        ra = torch.where(a == 0, torch.zeros_like(a), r * a)
+        fit = r.clamp(0.8, 1.2) * a
+        slope = torch.where(ra <= fit, -ra, torch.zeros_like(a)) + kl * (1 - u.exp())
+        gh = -entropy_coef * w if entropy_coef else None
+        want, bound = reference_grad(logits, targets, 1.0, slope * w.double(), gh)
+        size = torch.where(ra <= fit, ra.abs(), torch.zeros_like(a)) + kl * (1 + u.exp())
+        _, p, _ = softmax64(logits, 1.0)
+        hot = torch.zeros_like(p).scatter_(1, targets.long()[:, None], 1.0)
+        close(out.grad, want, bound + (size * w.double() * LP_ATOL * 1.1)[:, None] * (hot + p), "grad")
+        row = -torch.minimum(ra, fit) + kl * (u.exp() - u - 1) - entropy_coef * h
+        row = torch.where(row > torch.finfo(torch.float32).max, math.inf, row)
+        tol = (torch.minimum(ra, fit).abs() + kl * (1 + u.exp())) * LP_ATOL * 1.1 + entropy_coef * H_ATOL
+        fits = ~torch.isinf(row)
+        close(out.row_loss, torch.where(fits, row, row), torch.where(fits, tol, torch.zeros_like(tol)), "row_loss")
+        w = torch.where(fits, w, torch.zeros_like(w))
+        out = q().policy_loss(logits, targets, old, adv, weight=w, **kw)
+        part = torch.where(fits, row, torch.zeros_like(row)) * w.double()
+        lim = torch.where(fits, tol * w.double(), torch.zeros_like(tol)).sum() + part.abs().sum() * EPS
+        close(out.loss, part.sum(), lim.item(), "loss")
+    bad = old.clone()
+    bad[0] = math.nan  # no ratio at all
+    out = q().policy_loss(logits, targets, bad, adv, entropy_coef=entropy_coef)
+    assert torch.isnan(out.row_loss[0]) and torch.isnan(out.grad[0]).all() and torch.isfinite(out.grad[1].float()).all()
+
+
+@pytest.mark.parametrize("entropy", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", RANGES, ids=str)
+def test_infinite_derivatives(shape, dtype, entropy):
+    """A derivative that is infinite, or beyond fp32: infinities with their signs where the probability is not 0, zeros
+    where it is, and no NaN."""
+    rows, V = shape
+    logits, targets, g = banned_rows(rows, V, dtype, 81)
+    lp, _ = reference(logits, targets, 1.0)
+    hot = torch.zeros(rows, V, dtype=torch.bool, device="cuda").scatter_(1, targets.long()[:, None], True)
+
+    def check(grad, sign):
+        zero = (logits == -math.inf) & ~hot
+        assert (grad[zero] == 0).all()
+        assert (grad[hot] == sign * math.inf).all()
+        assert (grad[~hot & ~zero] == -sign * math.inf).all()
+
+    coef = 0.01 if entropy else 0.0
+    one = torch.ones(rows, device="cuda")
+    out = q().policy_loss(logits, targets, (lp - 110).float(), -one, weight=one, entropy_coef=coef)
+    check(out.grad, 1)
+    fwd = q().token_logprobs(logits, targets, entropy=True)
+    kw = dict(entropy=fwd.entropy, grad_entropy=one) if entropy else {}
+    check(q().token_logprobs_grad(logits, targets, fwd.stats, math.inf * one, **kw), 1)
+    check(q().token_logprobs_grad(logits, targets, fwd.stats, -math.inf * one, **kw), -1)
+    logits.masked_fill_(hot, -math.inf)  # a target of probability 0 under a reference that allows it
+    out = q().policy_loss(logits, targets, -3 * one, one, ref_logprob=-3 * one, kl_coef=0.1, entropy_coef=coef)
+    assert out.loss.item() == math.inf and (out.row_loss == math.inf).all()
+    check(out.grad, -1)
