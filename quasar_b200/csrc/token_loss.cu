@@ -1214,7 +1214,7 @@ __device__ __forceinline__ double pair_loss(const PairArgs& p, int i, int tid, d
     if (ok) {
         for (int s = 0; s < 2; s++) {
             double x = 0.0, c = 0.0;
-            for (int64_t r = at[s] + tid; r < at[s + 1]; r += NT)
+            for (int64_t r = (int64_t)at[s] + tid; r < at[s + 1]; r += NT)
                 if (p.targets[r] >= 0) x += (double)p.logprob[r], c += 1.0;
             sum[s] = WARP ? warp_sum(x) : cta_sum(x, buf, NT);
             n[s] = WARP ? warp_sum(c) : cta_sum(c, buf, NT);
@@ -1243,7 +1243,7 @@ __device__ __forceinline__ double pair_loss(const PairArgs& p, int i, int tid, d
     }
     if (ok)
         for (int s = 0; s < 2; s++)
-            for (int64_t r = at[s] + tid; r < at[s + 1]; r += NT)
+            for (int64_t r = (int64_t)at[s] + tid; r < at[s + 1]; r += NT)
                 if (p.targets[r] >= 0) p.row_grad[r] = (float)((s ? -g : g) * by[s]);
     return loss;
 }

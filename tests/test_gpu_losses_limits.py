@@ -105,3 +105,19 @@ def test_infinite_derivatives(shape, dtype, entropy):
     out = q().policy_loss(logits, targets, -3 * one, one, ref_logprob=-3 * one, kl_coef=0.1, entropy_coef=coef)
     assert out.loss.item() == math.inf and (out.row_loss == math.inf).all()
     check(out.grad, -1)
+
+
+def test_sequences_at_the_last_rows_of_31_bits():
+    """Sequences whose first row is within a CTA's threads of 2^31: V = 1, so that every log-probability is 0, the loss
+    is ln 2 and a row's derivative beta / 2."""
+    rows = (1 << 31) - 1
+    logits = torch.zeros(rows, 1, dtype=torch.float16, device="cuda")
+    targets = torch.zeros(rows, dtype=torch.int32, device="cuda")
+    cu = torch.tensor([rows - 180, rows - 120, rows - 20], dtype=torch.int32, device="cuda")
+    out = q().preference_loss(logits, targets, cu, grad=False)
+    assert (out.seq_logprob == 0).all() and abs(out.loss.item() - math.log(2)) <= EPS
+    end = out.row_grad[rows - 200:]
+    assert (end[:20] == 0).all() and (end[180:] == 0).all()
+    half = torch.tensor(0.1, dtype=torch.float32, device="cuda") / 2  # beta is an fp32 parameter
+    assert (end[20:80] == -half).all() and (end[80:180] == half).all()
+    assert int(out.row_grad.count_nonzero()) == 160
