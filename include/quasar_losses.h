@@ -167,6 +167,20 @@ int quasar_preference_loss(const void *d_logits, int dtype, int64_t ld, int rows
                            quasar_logprob_stat *d_stats, float *d_row_grad,
                            void *d_grad, int64_t grad_ld, void *stream);
 
+/* ---- self-test ------------------------------------------------------------ */
+
+/* quasar_policy_loss with waits of at most wait_cycles (0 to 2^32), of which
+ * one CTA's loads stop after `chunks` chunks where the call takes the streaming
+ * kernel (many long rows, with d_grad): waits run out there. Used by the GPU
+ * tests to see that what was not computed comes out NaN. */
+int quasar_selftest_stalled_policy_loss(int64_t wait_cycles, int chunks,
+                                        const void *d_logits, int dtype, int64_t ld, int rows, int V,
+                                        const int32_t *d_targets, const float *d_old_logprob, const float *d_advantage,
+                                        const float *d_ref_logprob, const float *d_weight,
+                                        const quasar_policy_params *params,
+                                        float *d_logprob, float *d_entropy, float *d_row_loss, float *d_loss,
+                                        void *d_grad, int64_t grad_ld, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

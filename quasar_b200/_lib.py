@@ -67,6 +67,8 @@ SIGNATURES = {
     "quasar_token_logprobs": ([_P, _I, _I64, _I, _I, _P, _F, _P, _P, _P, _P], _I),
     "quasar_token_logprobs_grad": ([_P, _I, _I64, _I, _I, _P, _F, _P, _P, _P, _P, _P, _I64, _P], _I),
     "quasar_policy_loss": ([_P, _I, _I64, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _P], _I),
+    "quasar_selftest_stalled_policy_loss": ([_I64, _I, _P, _I, _I64, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _P],
+                                            _I),
     "quasar_preference_loss": ([_P, _I, _I64, _I, _I, _P, _P, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64,
                                 _P], _I),
 }

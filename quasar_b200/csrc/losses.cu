@@ -4,6 +4,7 @@
 #include <string.h>
 
 #include "../../include/quasar_losses.h"
+#include "ptx.cuh"
 #include "token_loss.cuh"
 
 namespace {
@@ -41,10 +42,50 @@ qs::loss::Args row_args(const void* d_logits, int64_t ld, int rows, int V, const
     a.targets = d_targets;
     a.inv_t = 1.0 / (double)temperature;
     a.k = (float)(1.4426950408889634074 * a.inv_t);
+    a.wait = qs::WAIT_CYCLES;
+    a.stall = -1;
     return a;
 }
 
 int status(cudaError_t e) { return e == cudaSuccess ? QUASAR_OK : QUASAR_ECUDA; }
+
+int policy_loss(int64_t wait, int stall, const void* d_logits, int dtype, int64_t ld, int rows, int V, const int32_t* d_targets,
+                const float* d_old_logprob, const float* d_advantage, const float* d_ref_logprob,
+                const float* d_weight, const quasar_policy_params* params, float* d_logprob, float* d_entropy,
+                float* d_row_loss, float* d_loss, void* d_grad, int64_t grad_ld, void* stream) {
+    if (!params || !d_loss) return QUASAR_EINVAL;
+    if (!check_rows(d_logits, dtype, ld, rows, V, d_targets, params->temperature)) return QUASAR_EINVAL;
+    if (!(params->clip_low >= 0.0f) || !(params->clip_high >= 0.0f) || !isfinite(params->kl_coef) ||
+        !isfinite(params->entropy_coef) || !isfinite(params->grad_scale))
+        return QUASAR_EINVAL;
+    if (d_grad && !check_grad(d_logits, dtype, ld, rows, V, d_grad, grad_ld)) return QUASAR_EINVAL;
+    const cudaStream_t st = (cudaStream_t)stream;
+    if (rows > 0) {
+        if (!d_old_logprob || !d_advantage || !d_logprob || !d_row_loss) return QUASAR_EINVAL;
+        if (params->kl_coef != 0.0f && !d_ref_logprob) return QUASAR_EINVAL;
+        qs::loss::Args a = row_args(d_logits, ld, rows, V, d_targets, params->temperature);
+        a.logprob = d_logprob;
+        a.entropy = d_entropy;
+        a.old_lp = d_old_logprob;
+        a.adv = d_advantage;
+        a.ref_lp = d_ref_logprob;
+        a.weight = d_weight;
+        a.mean = 1.0 / rows;
+        a.clip_lo = params->clip_low;
+        a.clip_hi = params->clip_high;
+        a.kl = params->kl_coef;
+        a.ec = params->entropy_coef;
+        a.row_loss = d_row_loss;
+        a.scale = params->grad_scale;
+        a.grad = d_grad;
+        a.grad_ld = grad_ld;
+        a.wait = wait;
+        a.stall = stall;
+        const int rc = status(qs::loss::launch_rows(a, dtype, st));
+        if (rc != QUASAR_OK) return rc;
+    }
+    return status(qs::loss::launch_weighted_sum(d_row_loss, d_weight, rows, d_loss, st));
+}
 
 }  // namespace
 
@@ -85,36 +126,18 @@ int quasar_policy_loss(const void* d_logits, int dtype, int64_t ld, int rows, in
                        const float* d_old_logprob, const float* d_advantage, const float* d_ref_logprob,
                        const float* d_weight, const quasar_policy_params* params, float* d_logprob, float* d_entropy,
                        float* d_row_loss, float* d_loss, void* d_grad, int64_t grad_ld, void* stream) {
-    if (!params || !d_loss) return QUASAR_EINVAL;
-    if (!check_rows(d_logits, dtype, ld, rows, V, d_targets, params->temperature)) return QUASAR_EINVAL;
-    if (!(params->clip_low >= 0.0f) || !(params->clip_high >= 0.0f) || !isfinite(params->kl_coef) ||
-        !isfinite(params->entropy_coef) || !isfinite(params->grad_scale))
-        return QUASAR_EINVAL;
-    if (d_grad && !check_grad(d_logits, dtype, ld, rows, V, d_grad, grad_ld)) return QUASAR_EINVAL;
-    const cudaStream_t st = (cudaStream_t)stream;
-    if (rows > 0) {
-        if (!d_old_logprob || !d_advantage || !d_logprob || !d_row_loss) return QUASAR_EINVAL;
-        if (params->kl_coef != 0.0f && !d_ref_logprob) return QUASAR_EINVAL;
-        qs::loss::Args a = row_args(d_logits, ld, rows, V, d_targets, params->temperature);
-        a.logprob = d_logprob;
-        a.entropy = d_entropy;
-        a.old_lp = d_old_logprob;
-        a.adv = d_advantage;
-        a.ref_lp = d_ref_logprob;
-        a.weight = d_weight;
-        a.mean = 1.0 / rows;
-        a.clip_lo = params->clip_low;
-        a.clip_hi = params->clip_high;
-        a.kl = params->kl_coef;
-        a.ec = params->entropy_coef;
-        a.row_loss = d_row_loss;
-        a.scale = params->grad_scale;
-        a.grad = d_grad;
-        a.grad_ld = grad_ld;
-        const int rc = status(qs::loss::launch_rows(a, dtype, st));
-        if (rc != QUASAR_OK) return rc;
-    }
-    return status(qs::loss::launch_weighted_sum(d_row_loss, d_weight, rows, d_loss, st));
+    return policy_loss(qs::WAIT_CYCLES, -1, d_logits, dtype, ld, rows, V, d_targets, d_old_logprob, d_advantage, d_ref_logprob,
+                       d_weight, params, d_logprob, d_entropy, d_row_loss, d_loss, d_grad, grad_ld, stream);
+}
+
+int quasar_selftest_stalled_policy_loss(int64_t wait_cycles, int chunks, const void* d_logits, int dtype, int64_t ld, int rows, int V,
+                       const int32_t* d_targets,
+                       const float* d_old_logprob, const float* d_advantage, const float* d_ref_logprob,
+                       const float* d_weight, const quasar_policy_params* params, float* d_logprob, float* d_entropy,
+                       float* d_row_loss, float* d_loss, void* d_grad, int64_t grad_ld, void* stream) {
+    if (wait_cycles < 0 || wait_cycles > qs::WAIT_CYCLES || chunks < 0) return QUASAR_EINVAL;
+    return policy_loss(wait_cycles, chunks, d_logits, dtype, ld, rows, V, d_targets, d_old_logprob, d_advantage, d_ref_logprob,
+                       d_weight, params, d_logprob, d_entropy, d_row_loss, d_loss, d_grad, grad_ld, stream);
 }
 
 int quasar_preference_loss(const void* d_logits, int dtype, int64_t ld, int rows, int V, const int32_t* d_targets,

@@ -238,7 +238,7 @@ __device__ __forceinline__ void acc_one(Acc& a, float x, float k) {
 
 // (max, sum, Q) of a set of elements, the sums against the scaled maximum.
 struct __align__(16) Part {
-    float m, s, q, pad;
+    float m, s, q, tag;
 };
 
 // The reference of sums with maximum m (finite for a maximum of the lowest
@@ -264,7 +264,7 @@ __device__ __forceinline__ Part warp_part(const Acc& a, float k) {
     rebase(s0, q0, a.c, p.m, k);
     p.s = warp_sum(s0);
     p.q = ENT ? warp_sum(q0) : 0.0f;
-    p.pad = 0.0f;
+    p.tag = 0.0f;
     return p;
 }
 
@@ -564,8 +564,9 @@ __device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
     return r;
 }
+__device__ __forceinline__ void remote_store(uint32_t addr, int x) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(x) : "memory"); }
 __device__ __forceinline__ void remote_store(uint32_t addr, const Part& p) {
-    asm volatile("st.shared::cluster.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "f"(p.m), "f"(p.s), "f"(p.q), "f"(p.pad) : "memory");
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "f"(p.m), "f"(p.s), "f"(p.q), "f"(p.tag) : "memory");
 }
 
 // Sums of one thread's share of a slice against M itself, with differences
@@ -789,6 +790,7 @@ struct StreamShared {
     Part own[2][Shape::NW];   // of the rows in turn, from the CTA's warps
     Part parts[2][MAXC];      // ... and from the cluster's CTAs
     Part wide_parts[MAXC];
+    int sent[MAXC], wide_sent[MAXC];  // how many of them each CTA has sent here, at the end
     uint64_t full[Shape::STAGES], empty[Shape::STAGES];
     uint64_t obar[2], xbar[2], cbar[2], wbar;  // own parts, parts, coefficients, wide parts are here
     Coef coef[2];
@@ -802,22 +804,30 @@ struct StreamShared {
 __device__ __forceinline__ void send_part(uint32_t addr, uint32_t bar, const Part& p) {
     asm volatile(
         "st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1,%2,%3,%4}, [%5];" ::"r"(addr), "f"(p.m),
-        "f"(p.s), "f"(p.q), "f"(p.pad), "r"(bar)
+        "f"(p.s), "f"(p.q), "f"(p.tag), "r"(bar)
         : "memory");
 }
 
-// Waits for a phase of `bar`. After WAIT_CYCLES, or once another wait of the
+// Waits for a phase of `bar`. After `limit` cycles, or once another wait of the
 // CTA has given up, returns all the same: the CTA's rows then come out NaN.
-__device__ __forceinline__ void stream_wait(uint32_t bar, uint32_t parity, volatile int* abort) {
+__device__ __forceinline__ void stream_wait(uint32_t bar, uint32_t parity, volatile int* abort, long long limit) {
     if (mbar_try_wait(bar, parity)) return;
     const long long t0 = clock64();
     while (!mbar_try_wait(bar, parity)) {
         if (*abort) return;
-        if (clock64() - t0 > WAIT_CYCLES) {
+        if (clock64() - t0 > limit) {
             *abort = 1;
             return;
         }
     }
+}
+
+// Waits until the part with this tag has landed (0: none was sent).
+__device__ __forceinline__ void wait_landed(const Part& p, int tag) {
+    const volatile float* at = &p.tag;
+    const long long t0 = clock64();
+    while (tag > 0 && __float_as_int(*at) != tag)
+        if (clock64() - t0 > WAIT_CYCLES) return;
 }
 
 __device__ __forceinline__ uint4 lds_pack(uint32_t addr) {
@@ -874,6 +884,7 @@ __global__ void __launch_bounds__(Shape::NT + 64, Shape::CTAS) stream_kernel(con
             mbar_init(cbar_u + 8 * i, 1);
         }
         mbar_init(wbar_u, 1);
+        for (int i = 0; i < MAXC; i++) sh.parts[0][i].tag = sh.parts[1][i].tag = sh.wide_parts[i].tag = 0.0f;
         sh.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -905,11 +916,13 @@ __global__ void __launch_bounds__(Shape::NT + 64, Shape::CTAS) stream_kernel(con
             asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(again));
             asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(once));
             uint32_t stage = 0, phase = 0, issued = 0;
+            const uint32_t stop = cid == 0 && rank == C - 1 ? (uint32_t)a.stall : ~0u;
             const uint4* b_src = nullptr;  // the row before, whose gradient is due
             int b_n = 0, b_packs = 0;
             const auto put = [&](const uint4* src, int j, int packs, uint64_t pol) {
                 const uint32_t bytes = (uint32_t)min(CHP, packs - j * CHP) * 16;
-                stream_wait(empty_u + 8 * stage, phase ^ 1, abort);
+                if (issued == stop) return;
+                stream_wait(empty_u + 8 * stage, phase ^ 1, abort, a.wait);
                 if (*abort) return;
                 mbar_arrive_tx(full_u + 8 * stage, bytes);
                 bulk_load(ring_u + stage * CH, src + j * CHP, bytes, full_u + 8 * stage, pol);
@@ -934,18 +947,18 @@ __global__ void __launch_bounds__(Shape::NT + 64, Shape::CTAS) stream_kernel(con
                 }
                 b_src = src, b_n = n, b_packs = packs;
             }
-            if (*abort) {  // let the copies in flight land
-                const uint32_t n = min(issued, STAGES);
-                for (uint32_t i = 0; i < n; i++) {
-                    if (stage == 0) stage = STAGES, phase ^= 1;
-                    stage--;
-                    mbar_wait(full_u + 8 * stage, phase);
-                }
+            // the copies in flight land before the CTA leaves, whoever has given up
+            const uint32_t n = min(issued, STAGES);
+            for (uint32_t i = 0; i < n; i++) {
+                if (stage == 0) stage = STAGES, phase ^= 1;
+                stage--;
+                mbar_wait(full_u + 8 * stage, phase);
             }
         }
     } else if (warp == NW + 1) {  // ---- the joining warp: sums to coefficients
         uint32_t phases = 0;  // of xbar and obar, a bit for each parity
         uint32_t wphase = 0;
+        int sent = 0, wide_sent = 0;  // parts that this lane has sent to its peer, each with its number as tag
         const auto inputs = [&](int64_t r) {
             RowIn in{0.0f, 0.0f, 0.0f, 0.0f, 0.0};
             in.lt = widen1(((const T*)a.logits + r * a.ld)[a.targets[r]]);
@@ -966,25 +979,32 @@ __global__ void __launch_bounds__(Shape::NT + 64, Shape::CTAS) stream_kernel(con
                 next = nth_row(sh, a.rows, cid + (i + 1) * step, false);
                 next_in = inputs(next);
             }
-            stream_wait(obar_u + 8 * par, (phases >> par) & 1, abort);
+            stream_wait(obar_u + 8 * par, (phases >> par) & 1, abort, a.wait);
             Row w = join_parts<ENT>(sh.own[par], NW, k);
             if (C > 1) {
-                if (lane == 0) mbar_arrive_tx(xbar_u + 8 * par, C * 16);
+                // nothing is sent, and no barrier armed again, once a wait has given up
+                if (lane == 0 && !*abort) mbar_arrive_tx(xbar_u + 8 * par, C * 16);
                 __syncwarp();
-                if (lane < C && !*abort)
-                    send_part(map_rank(smem_u32(&sh.parts[par][rank]), lane), map_rank(xbar_u + 8 * par, lane), Part{w.M, (float)w.S, (float)w.Q, 0.0f});
-                stream_wait(xbar_u + 8 * par, (phases >> par) & 1, abort);
+                if (lane < C && !*abort) {
+                    sent = i + 1;
+                    send_part(map_rank(smem_u32(&sh.parts[par][rank]), lane), map_rank(xbar_u + 8 * par, lane),
+                              Part{w.M, (float)w.S, (float)w.Q, __int_as_float(sent)});
+                }
+                stream_wait(xbar_u + 8 * par, (phases >> par) & 1, abort, a.wait);
                 w = join_parts<ENT>(sh.parts[par], C, k);
             }
             phases ^= 1u << par;
             if (*abort) w.S = NAN, w.wide = false;
             if (w.wide) {  // the same in every CTA: once more through the slices, by these warps
                 const T* row = (const T*)a.logits + r * a.ld;
-                const Part own = wide_part<T, ENT>(row, a.V, w.M, k, rank, C, lane, 32);
-                if (lane == 0) mbar_arrive_tx(wbar_u, C * 16);
+                Part own = wide_part<T, ENT>(row, a.V, w.M, k, rank, C, lane, 32);
+                if (lane == 0 && !*abort) mbar_arrive_tx(wbar_u, C * 16);
                 __syncwarp();
-                if (lane < C && !*abort) send_part(map_rank(smem_u32(&sh.wide_parts[rank]), lane), map_rank(wbar_u, lane), own);
-                stream_wait(wbar_u, wphase, abort);
+                if (lane < C && !*abort) {
+                    own.tag = __int_as_float(++wide_sent);
+                    send_part(map_rank(smem_u32(&sh.wide_parts[rank]), lane), map_rank(wbar_u, lane), own);
+                }
+                stream_wait(wbar_u, wphase, abort, a.wait);
                 wphase ^= 1;
                 w = join_wide(sh.wide_parts, C, w.M, k);
                 if (*abort) w.S = NAN;
@@ -996,6 +1016,10 @@ __global__ void __launch_bounds__(Shape::NT + 64, Shape::CTAS) stream_kernel(con
                 if (rank == 0) write_row<ENT, true>(a, r, w, in);
             }
             __syncwarp();
+        }
+        if (C > 1 && lane < C) {
+            remote_store(map_rank(smem_u32(&sh.sent[rank]), lane), sent);
+            remote_store(map_rank(smem_u32(&sh.wide_sent[rank]), lane), wide_sent);
         }
     } else {  // ---- the consumers
         uint32_t stage = 0, phase = 0, cphase = 0;
@@ -1015,7 +1039,7 @@ __global__ void __launch_bounds__(Shape::NT + 64, Shape::CTAS) stream_kernel(con
             float edge = -INFINITY;
             int n = 0;
             if (more) {  // the row's number comes with its first chunk
-                stream_wait(full_u + 8 * stage, phase, abort);
+                stream_wait(full_u + 8 * stage, phase, abort, a.wait);
                 r = *abort ? nth_row(sh, a.rows, cid + i * step, false) : *(volatile int*)&sh.rows[i & 7];
                 row = (const T*)a.logits + r * a.ld;
                 s = slice_of(row, a.V, rank, C, tid);
@@ -1030,7 +1054,7 @@ __global__ void __launch_bounds__(Shape::NT + 64, Shape::CTAS) stream_kernel(con
             const bool same = ((uintptr_t)b_dst & 15) == 0;
             const auto want_c = [&]() {  // the coefficients of the row before
                 if (have_c) return;
-                stream_wait(cbar_u + 8 * (par ^ 1), (cphase >> (par ^ 1)) & 1, abort);
+                stream_wait(cbar_u + 8 * (par ^ 1), (cphase >> (par ^ 1)) & 1, abort, a.wait);
                 cphase ^= 1u << (par ^ 1);
                 c = sh.coef[par ^ 1];
                 if (*abort) c.kind = ROW_NAN;
@@ -1038,7 +1062,7 @@ __global__ void __launch_bounds__(Shape::NT + 64, Shape::CTAS) stream_kernel(con
             };
             for (int j = 0; j < steps; j++) {
                 if (j < n) {
-                    stream_wait(full_u + 8 * stage, phase, abort);
+                    stream_wait(full_u + 8 * stage, phase, abort, a.wait);
                     const uint32_t at = ring_u + stage * CH + tid * 16;
                     uint4 p[PP];
                     if (j + 1 < n) {
@@ -1069,7 +1093,7 @@ __global__ void __launch_bounds__(Shape::NT + 64, Shape::CTAS) stream_kernel(con
                 if (j >= lag && j - lag < b_n) {
                     want_c();
                     const int base = (j - lag) * CHP + tid;
-                    stream_wait(full_u + 8 * stage, phase, abort);
+                    stream_wait(full_u + 8 * stage, phase, abort, a.wait);
                     const uint32_t at = ring_u + stage * CH + tid * 16;
                     uint4* d = reinterpret_cast<uint4*>(b_dst) + base;
                     if (same && c.kind == ROW_SUM && j - lag + 1 < b_n) {
@@ -1118,11 +1142,19 @@ __global__ void __launch_bounds__(Shape::NT + 64, Shape::CTAS) stream_kernel(con
             grad_plain<T, ENT>(row, out, s.head, 0, s.n, c, k, tid, NT);
         }
     }
-    // no CTA leaves while a peer may still store into its shared memory
+    // no CTA leaves while a peer may still store into its shared memory, or
+    // while a part is on its way to it: those of rows that it has joined have
+    // landed, and where its waits gave up, the last two rows' may not have
     __syncwarp();
     launch_next();
     cluster_arrive();
     cluster_wait();
+    if (*abort && C > 1 && warp == NW + 1 && lane < C) {
+        const int n = sh.sent[lane];
+        wait_landed(sh.parts[(n + 1) & 1][lane], n);
+        wait_landed(sh.parts[n & 1][lane], n - 1);
+        wait_landed(sh.wide_parts[lane], sh.wide_sent[lane]);
+    }
 }
 
 // ---- the gradient from given sums -------------------------------------------------

@@ -42,6 +42,11 @@ struct Args {
     const float* g_ent;      // ... or NULL
     const float* ent_in;     // entropies the statistics kernel gave (with g_ent)
     const quasar_logprob_stat* stats_in;
+
+    // streaming kernel: the limit of a wait in cycles, and for the self-test
+    // the chunks after which one CTA's loads stop (-1: they do not)
+    long long wait;
+    int stall;
 };
 
 struct PairArgs {

@@ -121,3 +121,54 @@ def test_sequences_at_the_last_rows_of_31_bits():
     half = torch.tensor(0.1, dtype=torch.float32, device="cuda") / 2  # beta is an fp32 parameter
     assert (end[20:80] == -half).all() and (end[80:180] == half).all()
     assert int(out.row_grad.count_nonzero()) == 160
+
+
+# rows, V, dtype, with entropy, chunks that the stalled CTA gets: none, in the first row's sums, between its sums and its
+# gradient, in a later row; rows of one CTA, of two, and of eight
+STALLS = [(600, 30001, torch.float32, False, (0, 1, 5, 9, 16)), (700, 60001, torch.float16, True, (3, 8, 13)),
+          (300, 75001, torch.float32, False, (0, 2, 6, 8, 11, 17, 30)), (450, 151936, torch.bfloat16, True, (3, 7, 9, 14, 22)),
+          (60 + 148, 1 << 20, torch.float32, False, (5, 19, 21, 30, 60))]
+
+
+def stalled_calls(case):
+    """The call whole, then with one CTA's loads stopped after so many chunks each time, then whole again: yields the
+    chunks and (logprob, row_loss, loss, grad), the buffers of all calls."""
+    rows, V, dtype, entropy, stops = case
+    from quasar_b200.losses import PolicyParams
+    logits, targets, g = rows_of(rows, V, dtype, 86)
+    old, adv = torch.full((rows,), -9.0, device="cuda"), torch.randn(rows, generator=g, device="cuda")
+    prm = PolicyParams(1.0, 0.2, 0.2, 0.0, 0.01 if entropy else 0.0, 64.0)
+    h = torch.empty(rows, device="cuda") if entropy else None
+    lp, row, loss, grad = (torch.empty(rows, device="cuda"), torch.empty(rows, device="cuda"), torch.empty((), device="cuda"),
+                           torch.empty_like(logits))
+    for chunks in (1 << 30, *stops, 1 << 30):
+        for t in (lp, row, loss, grad):
+            t.fill_(7.0)
+        rc = q().lib().quasar_selftest_stalled_policy_loss(
+            20_000_000, chunks, logits.data_ptr(), {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}[dtype], V, rows, V,
+            targets.data_ptr(), old.data_ptr(), adv.data_ptr(), None, None, ctypes.addressof(prm), lp.data_ptr(),
+            None if h is None else h.data_ptr(), row.data_ptr(), loss.data_ptr(), grad.data_ptr(), V,
+            torch.cuda.current_stream().cuda_stream)
+        assert rc == 0
+        torch.cuda.synchronize()
+        yield chunks, (lp, row, loss, grad)
+
+
+@pytest.mark.parametrize("case", STALLS, ids=lambda c: str(c[:4]))
+def test_waits_that_run_out(case):
+    """A CTA of the streaming kernel whose loads stop: its waits, and those of the CTAs that sum rows with it, run out
+    after 10 ms, and the call ends. Log-probabilities and losses are then as ever or NaN, and the next call is as ever."""
+    want = None
+    for chunks, out in stalled_calls(case):
+        lp, row, loss, grad = out
+        if chunks < 1 << 30:
+            for x, y in zip((lp, row), want):
+                assert bool(((x == y) | torch.isnan(x)).all()), f"{chunks} chunks"
+            assert int(torch.isnan(lp).sum()) <= case[0] // 8
+            assert torch.equal(torch.isnan(lp), torch.isnan(row)) and torch.isnan(loss) == torch.isnan(row).any()
+            assert torch.isnan(grad).any()
+        elif want is None:
+            want = [t.clone() for t in out]
+            assert torch.isfinite(grad.float()).all() and torch.isfinite(loss)
+        else:
+            assert all(torch.equal(x, y) for x, y in zip(out, want))
