@@ -12,6 +12,8 @@
  * after the launch. No call allocates, synchronises or keeps anything between
  * calls: every buffer, scratch included, is the caller's, so calls that use
  * different buffers may overlap and every call can be captured into a graph.
+ * A kernel's waits for its own copies and sums end after 2^32 cycles (about
+ * 2 s; they take microseconds): what was not computed by then comes out NaN.
  * Outputs are apart from inputs and from each other but where it says may be.
  * Results do not depend on the run: no sum is formed by atomics.
  *

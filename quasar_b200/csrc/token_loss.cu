@@ -809,17 +809,20 @@ __device__ __forceinline__ void send_part(uint32_t addr, uint32_t bar, const Par
 }
 
 // Waits for a phase of `bar`. After `limit` cycles, or once another wait of the
-// CTA has given up, returns all the same: the CTA's rows then come out NaN.
-__device__ __forceinline__ void stream_wait(uint32_t bar, uint32_t parity, volatile int* abort, long long limit) {
-    if (mbar_try_wait(bar, parity)) return;
+// CTA has given up, returns false: what the CTA has not computed by then comes
+// out NaN. (From then on a phase may be taken for another, so that a later wait
+// says true: rows are looked up by *abort as well.)
+__device__ __forceinline__ bool stream_wait(uint32_t bar, uint32_t parity, volatile int* abort, long long limit) {
+    if (mbar_try_wait(bar, parity)) return true;
     const long long t0 = clock64();
     while (!mbar_try_wait(bar, parity)) {
-        if (*abort) return;
+        if (*abort) return false;
         if (clock64() - t0 > limit) {
             *abort = 1;
-            return;
+            return false;
         }
     }
+    return true;
 }
 
 // Waits until the part with this tag has landed (0: none was sent).
@@ -1062,7 +1065,7 @@ __global__ void __launch_bounds__(Shape::NT + 64, Shape::CTAS) stream_kernel(con
             };
             for (int j = 0; j < steps; j++) {
                 if (j < n) {
-                    stream_wait(full_u + 8 * stage, phase, abort, a.wait);
+                    if (!stream_wait(full_u + 8 * stage, phase, abort, a.wait)) c.kind = ROW_NAN;
                     const uint32_t at = ring_u + stage * CH + tid * 16;
                     uint4 p[PP];
                     if (j + 1 < n) {
@@ -1093,7 +1096,7 @@ __global__ void __launch_bounds__(Shape::NT + 64, Shape::CTAS) stream_kernel(con
                 if (j >= lag && j - lag < b_n) {
                     want_c();
                     const int base = (j - lag) * CHP + tid;
-                    stream_wait(full_u + 8 * stage, phase, abort, a.wait);
+                    if (!stream_wait(full_u + 8 * stage, phase, abort, a.wait)) c.kind = ROW_NAN;
                     const uint32_t at = ring_u + stage * CH + tid * 16;
                     uint4* d = reinterpret_cast<uint4*>(b_dst) + base;
                     if (same && c.kind == ROW_SUM && j - lag + 1 < b_n) {
@@ -1119,9 +1122,11 @@ __global__ void __launch_bounds__(Shape::NT + 64, Shape::CTAS) stream_kernel(con
             if (i > 0) {
                 want_c();
                 if (b.edge >= 0) put_edge<T, ENT>(b_out, b.edge, b_target, b_edge, c, k);
-                // the thread that wrote the target's pack puts the target right
+                // the thread that wrote the target's pack puts the target right (NaN, too: its pack may
+                // be from before a wait gave up)
                 const int hot = b_target >= b.head ? (b_target - b.head) / N - b.lo : -1;
-                if (hot >= 0 && hot < b.n && hot % NT == tid && elementwise(c)) put1(b_out + b_target, grad_target<ENT>(c, c.lt, k));
+                if (hot >= 0 && hot < b.n && hot % NT == tid && c.kind != ROW_ZERO)
+                    put1(b_out + b_target, c.kind == ROW_NAN ? NAN : grad_target<ENT>(c, c.lt, k));
             }
             if (more) {
                 b_out = (T*)a.grad + r * a.grad_ld;

@@ -172,3 +172,17 @@ def test_waits_that_run_out(case):
             assert torch.isfinite(grad.float()).all() and torch.isfinite(loss)
         else:
             assert all(torch.equal(x, y) for x, y in zip(out, want))
+
+
+@pytest.mark.parametrize("case", STALLS, ids=lambda c: str(c[:4]))
+def test_gradients_behind_waits_that_run_out(case):
+    """The same call's gradients: every element as ever or NaN, NaN in rows of the stalled clusters alone."""
+    want = None
+    for chunks, (lp, row, loss, grad) in stalled_calls(case):
+        if want is None:
+            want = grad.clone()
+        elif chunks < 1 << 30:
+            lost = torch.isnan(grad).any(1)
+            assert 1 <= int(lost.sum()) <= case[0] // 8
+            assert not (torch.isnan(lp) & ~lost).any()
+            assert bool(((grad == want) | torch.isnan(grad)).all()), f"{chunks} chunks: neither as ever nor NaN"
