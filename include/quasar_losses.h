@@ -22,7 +22,9 @@
  * d_targets[r] is its token:
  *   target < 0      the row takes no part: its logits are not read, its
  *                   outputs are 0 and its gradient is a row of zeros;
- *   target >= V     the row's outputs and its gradient are NaN.
+ *   target >= V     the row's outputs and its gradient are NaN (the gradient
+ *                   zeros in a row of weight 0, in a pair that takes no part
+ *                   and outside of the sequences).
  * A logit of -inf has probability 0 (as banned tokens do). A row whose logits
  * are all -inf has no distribution: its log-probability is -inf, its entropy
  * 0 and its gradient zeros. NaN or +inf in a row that takes part makes that

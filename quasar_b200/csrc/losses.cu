@@ -185,6 +185,7 @@ int quasar_preference_loss(const void* d_logits, int dtype, int64_t ld, int rows
     if (rc == QUASAR_OK && rows > 0 && d_grad) {
         a.stats_in = d_stats;
         a.g_lp = d_row_grad;
+        a.zero_is_out = true;
         a.grad = d_grad;
         a.grad_ld = grad_ld;
         rc = status(qs::loss::launch_grad(a, dtype, st));

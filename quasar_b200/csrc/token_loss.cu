@@ -1185,7 +1185,7 @@ __global__ void __launch_bounds__(256, 6) grad_kernel(const Args a, const int pa
     const T* row = (const T*)a.logits + r * a.ld;
     T* out = (T*)a.grad + r * a.grad_ld;
     const Slice s = slice_of(row, a.V, part, ROWS == 1 ? parts : 1, tid);
-    Coef c = fill_coef(target >= a.V);
+    Coef c = fill_coef(target >= a.V && !(a.zero_is_out && g_lp == 0.0f));
     if (target >= 0 && target < a.V) {
         const float R = rintf(st.max * k);
         const bool wide = !(fabsf(R) < WIDE) && !isinf(st.max);

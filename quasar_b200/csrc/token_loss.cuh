@@ -42,6 +42,7 @@ struct Args {
     const float* g_ent;      // ... or NULL
     const float* ent_in;     // entropies the statistics kernel gave (with g_ent)
     const quasar_logprob_stat* stats_in;
+    bool zero_is_out;        // g_lp of 0: the row takes no part, whatever its target (preference loss)
 
     // streaming kernel: the limit of a wait in cycles, and for the self-test
     // the chunks after which one CTA's loads stop (-1: they do not)

@@ -186,3 +186,21 @@ def test_gradients_behind_waits_that_run_out(case):
             assert 1 <= int(lost.sum()) <= case[0] // 8
             assert not (torch.isnan(lp) & ~lost).any()
             assert bool(((grad == want) | torch.isnan(grad)).all()), f"{chunks} chunks: neither as ever nor NaN"
+
+
+def test_targets_out_of_range_that_take_no_part():
+    """Targets behind the vocabulary in a pair of weight 0, in a pair of offsets out of range and behind the last
+    sequence: NaN as log-probability, zeros as gradient. In a pair that takes part: NaN."""
+    logits, targets, g = rows_of(14, 50, torch.float32, 82)
+    cu = torch.tensor([0, 2, 4, 6, 8, 10, 12], dtype=torch.int32, device="cuda")
+    targets[5] = targets[13] = 50
+    w = torch.tensor([1.0, 0.0, 1.0], device="cuda")
+    out = q().preference_loss(logits, targets, cu, pair_weight=w)
+    assert torch.isnan(out.logprob[[5, 13]]).all() and torch.isnan(out.pair_loss[1])
+    assert torch.isfinite(out.loss) and torch.isfinite(out.grad).all()
+    assert (out.grad[4:8] == 0).all() and (out.grad[12:] == 0).all() and (out.grad[:4] != 0).all()
+    out = q().preference_loss(logits, targets, cu, pair_weight=torch.ones(3, device="cuda"))
+    assert torch.isnan(out.loss) and torch.isnan(out.grad[4:8]).all() and (out.grad[12:] == 0).all()
+    cu[3] = 99  # pair 1 ends behind the rows
+    out = q().preference_loss(logits, targets, cu)
+    assert torch.isnan(out.loss) and (out.grad[4:8] == 0).all()
