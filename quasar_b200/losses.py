@@ -7,7 +7,8 @@ them. A target below 0 marks a row that takes no part (outputs 0, a gradient of 
 
 Losses return their gradient into the logits with them, so one call is a forward and a backward
 pass; a model goes on from there with ``logits.backward(result.grad)``. Nothing is registered
-with autograd. Outputs are allocated on the stream of the call, or given (``out=``, ``grad=``)
+with autograd; tensors of the caller's that are written count as changed in place, so that a graph
+which saved them refuses its backward pass. Outputs are allocated on the stream of the call, or given (``out=``, ``grad=``)
 and used again. torch is used only for device memory and streams.
 """
 from __future__ import annotations
@@ -131,6 +132,11 @@ def _p(t):
     return None if t is None else t.data_ptr()
 
 
+def _wrote(torch, *tensors):
+    """Counts the call's writing into a caller's tensors as in-place changes, which autograd refuses to miss."""
+    torch.autograd.graph.increment_version([t for t in tensors if t is not None])
+
+
 def _on(torch, device, stream, tensors, call):
     """call(the C stream) with the logits' device and the stream of the call current, so that what it allocates belongs
     to that stream; keeps the call's tensors from being handed out again before the stream is done."""
@@ -175,6 +181,8 @@ def token_logprobs(logits, targets, *, temperature: float = 1.0, entropy: bool =
         check(lib().quasar_token_logprobs(logits.data_ptr(), dt, ld, rows, V, targets.data_ptr(), temperature,
                                           o.logprob.data_ptr(), _p(o.entropy), o.stats.data_ptr(), st),
               "quasar_token_logprobs")
+        if out is not None:
+            _wrote(torch, *out)
         return o
     return _on(torch, device, stream, (logits, targets, *(out or ())), call)
 
@@ -204,6 +212,8 @@ def token_logprobs_grad(logits, targets, stats, grad_logprob, *, entropy=None, g
         check(lib().quasar_token_logprobs_grad(logits.data_ptr(), dt, ld, rows, V, targets.data_ptr(), temperature,
                                                stats.data_ptr(), _p(entropy), grad_logprob.data_ptr(), _p(grad_entropy),
                                                g.data_ptr(), _ld(g), st), "quasar_token_logprobs_grad")
+        if out is not None:
+            _wrote(torch, out)
         return g
     return _on(torch, device, stream, (logits, targets, stats, grad_logprob, entropy, grad_entropy, out), call)
 
@@ -259,6 +269,10 @@ def policy_loss(logits, targets, old_logprob, advantage, *, ref_logprob=None, we
                                        advantage.data_ptr(), _p(ref_logprob), _p(weight), ctypes.addressof(prm),
                                        o.logprob.data_ptr(), _p(o.entropy), o.row_loss.data_ptr(), o.loss.data_ptr(),
                                        _p(g), 0 if g is None else _ld(g), st), "quasar_policy_loss")
+        if out is not None:
+            _wrote(torch, *o[:4], buf)
+        elif buf is not None:
+            _wrote(torch, buf)
         return o
     used = (logits, targets, old_logprob, advantage, ref_logprob, weight, buf, *(out or ()))
     return _on(torch, device, stream, used, call)
@@ -308,6 +322,10 @@ def preference_loss(logits, targets, cu_seqlens, *, ref_logprob=None, pair_weigh
                                            o.pair_loss.data_ptr(), o.loss.data_ptr(), o.stats.data_ptr(),
                                            o.row_grad.data_ptr(), _p(g), 0 if g is None else _ld(g), st),
               "quasar_preference_loss")
+        if out is not None:
+            _wrote(torch, *o[:6], buf)
+        elif buf is not None:
+            _wrote(torch, buf)
         return o
     used = (logits, targets, cu_seqlens, ref_logprob, pair_weight, buf, *(out or ()))
     return _on(torch, device, stream, used, call)

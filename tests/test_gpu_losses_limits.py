@@ -204,3 +204,34 @@ def test_targets_out_of_range_that_take_no_part():
     cu[3] = 99  # pair 1 ends behind the rows
     out = q().preference_loss(logits, targets, cu)
     assert torch.isnan(out.loss) and (out.grad[4:8] == 0).all()
+
+
+def test_autograd_sees_what_is_written():
+    """Gradients and outputs written into a caller's tensors count as in-place changes: a graph that saved them refuses
+    its backward pass instead of using what was written over."""
+    rows, V = 6, 300
+    x, targets, g = rows_of(rows, V, torch.float32, 83)
+    f = torch.zeros(rows, device="cuda")
+    cu = torch.tensor([0, 3, 6], dtype=torch.int32, device="cuda")
+    stats = q().token_logprobs(x, targets).stats
+    for call in (lambda t: q().token_logprobs_grad(t, targets, stats, f, out=t),
+                 lambda t: q().policy_loss(t, targets, f, f, grad=t),
+                 lambda t: q().preference_loss(t, targets, cu, grad=t)):
+        leaf = x.clone().requires_grad_(True)
+        logits = leaf.tanh()  # saves its output
+        call(logits.detach())
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            logits.backward(torch.ones_like(logits))
+        logits = leaf * 1.0   # saves nothing of it
+        call(logits.detach())
+        logits.backward(torch.ones_like(logits))
+    for make in (lambda **kw: q().token_logprobs(x, targets, entropy=True, **kw),
+                 lambda **kw: q().policy_loss(x, targets, f, f, entropy=True, grad=False, **kw),
+                 lambda **kw: q().preference_loss(x, targets, cu, grad=False, **kw)):
+        out = make()
+        before = [None if t is None else t._version for t in out]
+        make(out=out)
+        assert all(t is None or t._version > b for t, b in zip(out, before))
+    with torch.inference_mode():
+        buf = torch.empty_like(x)
+        assert q().policy_loss(x, targets, f, f, grad=buf).grad is buf
