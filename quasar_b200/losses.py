@@ -18,6 +18,7 @@ from typing import NamedTuple, Optional
 
 from ._lib import BF16, F16, F32, check, lib
 
+_INT_MAX = 2 ** 31 - 1
 _DTYPES = {}  # torch dtype -> the C constant; filled at the first call, torch being imported only then
 # the current stream's handle by device index, where torch has a way to it without a Stream object (2 us)
 _raw = None
@@ -78,6 +79,8 @@ def _rows(logits, targets):
     if not logits.is_cuda:
         raise ValueError("logits must be a CUDA tensor")
     rows, V = logits.shape
+    if rows > _INT_MAX or V > _INT_MAX:  # the C entry would take the low 32 bits
+        raise ValueError(f"logits have too many {'rows' if rows > _INT_MAX else 'columns'}: {rows} x {V}")
     ld, unit = logits.stride()
     if unit != 1 and V > 1:
         raise ValueError("logits must have unit column stride")
@@ -296,6 +299,8 @@ def preference_loss(logits, targets, cu_seqlens, *, ref_logprob=None, pair_weigh
     if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] % 2 == 0:
         raise ValueError("cu_seqlens must have 2 * pairs + 1 offsets")
     n = cu_seqlens.shape[0] - 1
+    if n // 2 > _INT_MAX:
+        raise ValueError(f"cu_seqlens has too many offsets: {n + 1}")
     _vec(cu_seqlens, "cu_seqlens", (n + 1,), torch.int32, device)
     if ref_logprob is not None:
         _vec(ref_logprob, "ref_logprob", (n,), f32, device)

@@ -235,3 +235,20 @@ def test_autograd_sees_what_is_written():
     with torch.inference_mode():
         buf = torch.empty_like(x)
         assert q().policy_loss(x, targets, f, f, grad=buf).grad is buf
+
+
+def test_sizes_beyond_32_bits_are_refused():
+    """More columns (or rows) than the C entries count: an error, not the first columns alone."""
+    wide = torch.empty(1, (1 << 32) + 16, dtype=torch.float16, device="cuda")
+    wide[:, :64] = 0
+    t, f = torch.zeros(1, dtype=torch.int32, device="cuda"), torch.zeros(1, device="cuda")
+    cu = torch.zeros(3, dtype=torch.int32, device="cuda")
+    for call in (lambda: q().token_logprobs(wide, t), lambda: q().policy_loss(wide, t, f, f, grad=False),
+                 lambda: q().preference_loss(wide, t, cu, grad=False)):
+        with pytest.raises(ValueError, match="columns"):
+            call()
+    rows = (1 << 32) + 2
+    tall, t = wide.view(-1, 1)[:rows], torch.empty(rows, dtype=torch.int32, device="cuda")
+    t[:64] = 0
+    with pytest.raises(ValueError, match="rows"):
+        q().token_logprobs(tall, t)
