@@ -47,7 +47,12 @@ qs::loss::Args row_args(const void* d_logits, int64_t ld, int rows, int V, const
     return a;
 }
 
-int status(cudaError_t e) { return e == cudaSuccess ? QUASAR_OK : QUASAR_ECUDA; }
+// A failed launch's error is this call's status, and not the next call's last error.
+int status(cudaError_t e) {
+    if (e == cudaSuccess) return QUASAR_OK;
+    cudaGetLastError();
+    return QUASAR_ECUDA;
+}
 
 int policy_loss(int64_t wait, int stall, const void* d_logits, int dtype, int64_t ld, int rows, int V, const int32_t* d_targets,
                 const float* d_old_logprob, const float* d_advantage, const float* d_ref_logprob,

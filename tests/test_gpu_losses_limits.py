@@ -252,3 +252,25 @@ def test_sizes_beyond_32_bits_are_refused():
     t[:64] = 0
     with pytest.raises(ValueError, match="rows"):
         q().token_logprobs(tall, t)
+
+
+def test_a_failed_launch_is_not_the_next_calls_error():
+    """A launch into a stream whose capture is already lost fails; the sampler's next call on another stream does not."""
+    cuda = ctypes.CDLL("libcuda.so.1")
+    rows, V = 64, 4096
+    logits, targets, g = rows_of(rows, V, torch.float32, 84)
+    rng = torch.arange(1, rows + 1, dtype=torch.int64, device="cuda")
+    out = q().token_logprobs(logits, targets)
+    q().pick_batch(logits, rng, params=dict(temperature=0.9))
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    handle, graph = ctypes.c_void_p(stream.cuda_stream), ctypes.c_void_p()
+    assert cuda.cuStreamBeginCapture_v2(handle, 2) == 0
+    assert cuda.cuStreamSynchronize(handle) != 0  # not allowed while it captures: the capture is lost
+    st = q().lib().quasar_token_logprobs(logits.data_ptr(), 0, V, rows, V, targets.data_ptr(), 1.0, out.logprob.data_ptr(),
+                                         None, None, handle)
+    assert cuda.cuStreamEndCapture(handle, ctypes.byref(graph)) != 0
+    assert st == -3, st  # QUASAR_ECUDA
+    ids = q().pick_batch(logits, rng, params=dict(temperature=0.9))
+    torch.cuda.synchronize()
+    assert ((ids >= 0) & (ids < V)).all()
