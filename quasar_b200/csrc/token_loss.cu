@@ -571,20 +571,27 @@ __device__ __forceinline__ void remote_store(uint32_t addr, const Part& p) {
 
 // Sums of one thread's share of a slice against M itself, with differences
 // taken before the multiply: for rows whose maximum is so large, or so low,
-// that l * k - R would keep nothing of t (a row masked throughout).
+// that l * k - R would keep nothing of t (a row masked throughout). Such rows
+// hold many equal terms, whose roundings share a sign: 64 of them are added in
+// 32 bits, then in 64.
 template <typename T, bool ENT>
 __device__ __noinline__ Part wide_part(const T* row, int V, float M, float k, int part, int parts, int first, int nt) {
     const Slice sl = slice_of(row, V, part, parts, 0);
     const int v0 = part == 0 ? 0 : sl.head + sl.lo * Type<T>::N, v1 = part == parts - 1 ? V : sl.head + (sl.lo + sl.n) * Type<T>::N;
-    float s = 0.0f, q = 0.0f;
+    double S = 0.0, Q = 0.0;
+    for (int v = v0 + first; v < v1;) {
+        float s = 0.0f, q = 0.0f;
+        const int end = v1 - v > 64 * nt ? v + 64 * nt : v1;
 #pragma unroll 4
-    for (int v = v0 + first; v < v1; v += nt) {
-        const float t = (widen1(row[v]) - M) * k;
-        const float e = ex2_approx(t);
-        s += e;
-        if (ENT) q = fmaf(e, fmaxf(t, -200.0f), q);
+        for (; v < end; v += nt) {
+            const float t = (widen1(row[v]) - M) * k;
+            const float e = ex2_approx(t);
+            s += e;
+            if (ENT) q = fmaf(e, fmaxf(t, -200.0f), q);
+        }
+        S += (double)s, Q += (double)q;
     }
-    return Part{M, warp_sum(s), ENT ? warp_sum(q) : 0.0f, 0.0f};
+    return Part{M, (float)warp_sum(S), ENT ? (float)warp_sum(Q) : 0.0f, 0.0f};
 }
 
 // Joins such parts.

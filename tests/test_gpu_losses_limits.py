@@ -274,3 +274,59 @@ def test_a_failed_launch_is_not_the_next_calls_error():
     ids = q().pick_batch(logits, rng, params=dict(temperature=0.9))
     torch.cuda.synchronize()
     assert ((ids >= 0) & (ids < V)).all()
+
+
+WIDE_ROWS = [(160, torch.float32), (300, torch.float32)]
+
+
+@pytest.mark.parametrize("rows,dtype", WIDE_ROWS)
+def test_sums_of_wide_rows(rows, dtype):
+    """Rows masked throughout by a value near -1.5e7, where logits stand a whole number apart, at the largest vocabulary:
+    millions of equal terms, whose roundings all have one sign. At most 64 of them are added in 32 bits (a lane's
+    partial sum), then in 64: 64 * 2^-24 for the additions, (4 + 3 |t|) 2^-24 for a term with |t| < 2, and 4 roundings
+    of parts and of the logarithm."""
+    V = 1 << 20
+    logits = torch.full((rows, V), -1.5e7 - 1, dtype=dtype, device="cuda")
+    logits[:, 12345] = -1.5e7
+    targets = torch.full((rows,), 777, dtype=torch.int32, device="cuda")
+    s = (V - 1) * math.exp(-1) + 1
+    lp, h = -1 - math.log(s), math.log(s) + (V - 1) * math.exp(-1) / s
+    bound = (64 + 10 + 4) * EPS
+    f = torch.full((rows,), -14.0, device="cuda")
+    ref = torch.full((rows,), lp, dtype=torch.float64, device="cuda"), torch.full((rows,), h, dtype=torch.float64, device="cuda")
+    for out in (q().token_logprobs(logits, targets, entropy=True),
+                q().policy_loss(logits, targets, f, f, entropy=True, grad=logits)):
+        close(out.logprob, ref[0], bound, "logprob")
+        close(out.entropy, ref[1], 4 * bound, "entropy")  # ln S, and the mean of t (under 2 in size) with S and Q off
+
+
+# rows, V, dtype, as policy loss with its gradient, additions of a thread's lane (two lanes a thread)
+ENTROPIES = [(2000, 1000, torch.float16, False, 16), (2000, 4099, torch.float32, False, 17), (64, 151936, torch.bfloat16, False, 38),
+             (600, 30001, torch.float32, True, 59), (600, 50021, torch.float16, True, 98), (400, 75001, torch.float32, True, 59),
+             (400, 151936, torch.bfloat16, True, 170)]
+
+
+@pytest.mark.parametrize("case", ENTROPIES, ids=str)
+def test_entropies(case):
+    """H = ln S - ln2 Q / S. A lane adds n terms in fp32, each addition off by up to half a step, of random sign: sqrt(n / 3)
+    half steps as standard deviation, of sums whose terms' t lie up to 20 over the lane's reference; at the worst one
+    lane holds the row's mass, and five such deviations bound 10^4 rows. A common error of the terms cancels in H, the
+    rest is at most (4 + 1.4 E|t|) half steps times the spread of ln p. Most rows spread their mass over lanes: their
+    errors' median is under a quarter of that. The mean error is ex2.approx's varying part (under 2e-7) and four
+    standard errors."""
+    rows, V, dtype, policy, n = case
+    logits, targets, g = rows_of(rows, V, dtype, 85)
+    lnp, p, t = softmax64(logits, 1.0)
+    h = -(p * lnp).sum(1)
+    et = (p * t.abs()).sum(1)
+    spread = (p * (lnp + h[:, None]).abs()).sum(1)
+    bound = EPS * (5 * math.sqrt(n / 3) * math.log(2) * (21 + et) + (4 + 1.4 * et) * spread) + h * EPS
+    f = torch.full((rows,), -9.0, device="cuda")
+    if policy:
+        out = q().policy_loss(logits, targets, f, f, entropy=True).entropy
+    else:
+        out = q().token_logprobs(logits, targets, entropy=True).entropy
+    err = out.double() - h
+    assert (err.abs() <= bound).all(), f"off by {err.abs().max().item():.3g}, {(err.abs() / bound).max().item():.3g} of the bound"
+    assert (err.abs().median() <= bound.median() / 4).all(), f"median {err.abs().median().item():.3g}"
+    assert err.mean().abs().item() <= 2e-7 + 4 * err.std().item() / math.sqrt(rows), f"mean {err.mean().item():.3g}"
