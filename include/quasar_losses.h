@@ -13,7 +13,9 @@
  * calls: every buffer, scratch included, is the caller's, so calls that use
  * different buffers may overlap and every call can be captured into a graph.
  * A kernel's waits for its own copies and sums end after 2^32 cycles (about
- * 2 s; they take microseconds): what was not computed by then comes out NaN.
+ * 2 s; they take microseconds). Where one does, the status is still that of the
+ * launch: rows whose sums were not complete by then come out NaN, and so do all
+ * gradients of the CTA that gave up.
  * Outputs are apart from inputs and from each other but where it says may be.
  * Results do not depend on the run: no sum is formed by atomics.
  *
@@ -38,9 +40,10 @@
  * log-probabilities, entropies and losses are formed in 64 bits from them and
  * rounded once; gradients are formed in 32 bits and rounded once to dtype. A row whose derivatives by
  * log-probability and entropy are both 0 (a clipped ratio) has a gradient of
- * zeros, whatever its logits. A derivative that is infinite or passes the fp32
- * range gives infinities with their signs where p is not 0, and zeros where it
- * is. */
+ * zeros, whatever its logits. A derivative by the log-probability that is
+ * infinite or passes 1e38 * temperature gives infinities with their signs where
+ * p is not 0, and zeros where it is (one by the entropy: nothing defined where p
+ * is not 0). */
 #ifndef QUASAR_LOSSES_H
 #define QUASAR_LOSSES_H
 
@@ -107,7 +110,8 @@ typedef struct {
  * (old and ref log-probabilities, advantages and weights are constants); a
  * ratio at a border counts as not clipped, and an advantage of 0 takes nothing
  * of a ratio, an infinite one either. Ratio and KL factor may pass the fp32
- * range as long as their products with weight and grad_scale do not.
+ * range (up to e^176) as long as their products with weight and grad_scale do
+ * not.
  *   d_old_logprob, d_advantage   [rows].
  *   d_ref_logprob   [rows], or NULL with kl_coef == 0.
  *   d_weight        [rows], or NULL for 1/rows each. A row of weight 0 takes

@@ -305,10 +305,11 @@ struct Coef {
     float lt;  // the target's logit
     int kind;  // ROW_*
 };
-// ROW_WIDE: c is M itself, t = (l - c) * k; ROW_STEEP: a or b is infinite. The
-// first three take their elements one by one.
-enum { ROW_SUM = 0, ROW_WIDE = 1, ROW_STEEP = 2, ROW_ZERO = 3, ROW_NAN = 4 };
+// ROW_WIDE: c is M itself, t = (l - c) * k, and elements of p = 0 have a gradient
+// of 0 whatever a and b (rows of infinite derivatives are taken so, too).
+enum { ROW_SUM = 0, ROW_ZERO = 1, ROW_NAN = 2, ROW_WIDE = 3 };
 
+constexpr float STEEP = 1e38f;  // a coefficient beyond this counts as infinite
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.402823466e38f; }
 
 // The gradient of g_lp * logprob + g_ent * entropy: p_v = 2^t / S and
@@ -323,16 +324,13 @@ __device__ __forceinline__ Coef make_coef(float M, float R, bool wide, float S, 
     o.b = w * (float)LN2 * g_ent;
     o.one = g_lp * inv_t;
     o.lt = 0.0f;
-    if (g_lp == 0.0f && g_ent == 0.0f)
-        o.kind = ROW_ZERO;
-    else if (S != S)
-        o.kind = ROW_NAN;
-    else if (M == -INFINITY)
-        o.kind = ROW_ZERO;
-    else if (o.a != o.a || o.b != o.b)
-        o.kind = ROW_NAN;
-    else
-        o.kind = wide ? ROW_WIDE : finite(o.a) && finite(o.b) ? ROW_SUM : ROW_STEEP;
+    o.kind = (g_lp == 0.0f && g_ent == 0.0f) || (M == -INFINITY && S == S) ? ROW_ZERO : wide ? ROW_WIDE : ROW_SUM;
+    if (!(fabsf(o.a) <= STEEP && fabsf(o.b) <= STEEP) && o.kind != ROW_ZERO) {
+        o.kind = o.a == o.a && o.b == o.b ? ROW_WIDE : ROW_NAN;  // NaN of S or of a derivative
+        o.c = M;
+        if (fabsf(o.a) > STEEP) o.a *= INFINITY;
+        if (fabsf(o.b) > STEEP) o.b *= INFINITY;
+    }
     return o;
 }
 // A row without an element-wise gradient.
@@ -342,6 +340,9 @@ __device__ __forceinline__ Coef fill_coef(bool nan) {
     o.kind = nan ? ROW_NAN : ROW_ZERO;
     return o;
 }
+
+// The target's logit as its gradient takes it: nothing beside an infinite derivative.
+__device__ __forceinline__ float target_logit(const Coef& c, float l) { return finite(c.one) ? l : -INFINITY; }
 
 struct RowIn {  // a row's inputs beside its logits
     float lt, adv, old_lp, ref_lp;
@@ -379,29 +380,30 @@ __device__ __forceinline__ F policy_slope(F lo, F hi, F kl, F adv, F ratio, F eu
     return (x <= y ? -x : y < x ? (F)0 : (F)NAN) - (kl != (F)0 ? kl * eu : (F)0);
 }
 
-// The same in 64 bits, times the row's weight: for rows whose ratio or KL
-// factor passes fp32 (differences of log-probabilities above 88), where slope
-// times weight may still fit.
-__device__ __noinline__ float steep_slope(double lo, double hi, double kl, float adv, double d, double u, double ws) {
-    double loss;
-    return (float)(policy_slope<double>(lo, hi, kl, adv, exp(d), expm1(u), &loss) * ws);
+// e^d * f * ws, where e^d passes the fp32 range (d up to 176) and the product
+// may not.
+__device__ __forceinline__ float steep(float d, float f, float ws) {
+    const float h = expf(0.5f * d);
+    return h * ws * f * h;
 }
 
 // A row's gradient coefficients. All the row's threads wait for them, so the
 // exponentials of differences of log-probabilities, which are near 1, are
-// expf's here (2^-23 relative); their 64-bit forms took 1.4 us, and are taken
-// where 32 bits overflow.
+// expf's here (2^-23 relative); their 64-bit forms took 1.4 us. Where ratio or
+// KL factor passes fp32, slope and weight are multiplied by halves of it.
 template <bool ENT>
 __device__ __forceinline__ Coef row_coef(const Args& a, const Row& w, const RowIn& in) {
     const double lp = row_logprob(a, w, in.lt);
     const double d = lp - (double)in.old_lp, u = a.kl != 0.0 ? (double)in.ref_lp - lp : 0.0;
     const float S = (float)w.S, ratio = expf((float)d), eu = a.kl != 0.0 ? expm1f((float)u) : 0.0f;
-    float loss;
-    const float ws = (float)(in.weight * a.scale);
-    float g = policy_slope<float>((float)(1.0 - a.clip_lo), (float)(1.0 + a.clip_hi), (float)a.kl, in.adv, ratio, eu, &loss) * ws;
-    if (!finite(g)) g = steep_slope(1.0 - a.clip_lo, 1.0 + a.clip_hi, a.kl, in.adv, d, u, in.weight * a.scale);
+    const float lo = (float)(1.0 - a.clip_lo), hi = (float)(1.0 + a.clip_hi), kl = (float)a.kl, ws = (float)(in.weight * a.scale);
+    float loss, g = policy_slope<float>(lo, hi, kl, in.adv, ratio, eu, &loss) * ws;
+    if (!finite(g) && d == d && u == u) {
+        const bool out = in.adv == 0.0f || (in.adv > 0.0f ? ratio > hi : ratio < lo);
+        g = (out ? 0.0f : -steep((float)d, in.adv, ws)) - (steep((float)u, kl, ws) - kl * ws);
+    }
     Coef c = make_coef(w.M, (float)w.R, w.wide, S, ENT ? (float)-LN2 * ((float)w.Q / S) : 0.0f, g, ENT ? -(float)a.ec * ws : 0.0f, (float)a.inv_t);
-    c.lt = in.lt;
+    c.lt = target_logit(c, in.lt);
     return c;
 }
 
@@ -448,13 +450,7 @@ template <bool ENT>
 __device__ __forceinline__ float grad1(const Coef& c, float l, float k) {
     const float t = c.kind == ROW_WIDE ? (l - c.c) * k : fmaf(l, k, -c.c);
     const float e = ex2_approx(t), f = ENT ? fmaf(c.b, fmaxf(t, -200.0f), c.a) : c.a;
-    return e == 0.0f && !finite(f) ? 0.0f : e * f;
-}
-
-// The target's: an infinite derivative stays what it is.
-template <bool ENT>
-__device__ __forceinline__ float grad_target(const Coef& c, float l, float k) {
-    return finite(c.one) ? grad1<ENT>(c, l, k) + c.one : c.one;
+    return c.kind == ROW_WIDE && e == 0.0f ? 0.0f : e * f;
 }
 
 // A pack's gradient (rows of ROW_SUM).
@@ -480,9 +476,9 @@ __device__ __forceinline__ uint4 grad_of(const uint4& p, const Coef& c, float k)
     return narrow(x, (T*)nullptr);
 }
 
-// The same for rows of the other kinds (rare: out of the streaming loops).
+// The same for rows of ROW_WIDE (rare: out of the streaming loops).
 template <typename T, bool ENT>
-__device__ __noinline__ uint4 grad_of_rare(uint4 p, Coef c, float k) {
+__device__ __noinline__ uint4 grad_of_wide(uint4 p, Coef c, float k) {
     float x[Type<T>::N];
     widen(p, x, (T*)nullptr);
 #pragma unroll
@@ -490,7 +486,7 @@ __device__ __noinline__ uint4 grad_of_rare(uint4 p, Coef c, float k) {
     return narrow(x, (T*)nullptr);
 }
 
-__device__ __forceinline__ bool elementwise(const Coef& c) { return c.kind <= ROW_STEEP; }
+__device__ __forceinline__ bool elementwise(const Coef& c) { return c.kind == ROW_SUM || c.kind == ROW_WIDE; }
 
 // A pack of zeros, or of NaN.
 template <typename T>
@@ -519,11 +515,12 @@ __device__ __noinline__ void store_elements(T* dst, uint4 p) {
 // An edge element's gradient.
 template <typename T, bool ENT>
 __device__ __forceinline__ void put_edge(T* out, int v, int target, float l, const Coef& c, float k) {
-    put1(out + v, c.kind == ROW_ZERO ? 0.0f : c.kind == ROW_NAN ? NAN : v == target ? grad_target<ENT>(c, l, k) : grad1<ENT>(c, l, k));
+    const bool hot = v == target;
+    put1(out + v, c.kind == ROW_ZERO ? 0.0f : c.kind == ROW_NAN ? NAN : grad1<ENT>(c, hot ? target_logit(c, l) : l, k) + (hot ? c.one : 0.0f));
 }
 
 // Writes a row's gradient where no batch loop fits: element-wise gradients of
-// rows of the rare kinds, fills, and rows of another 16-byte phase than the logits'.
+// wide rows, fills, and rows of another 16-byte phase than the logits'.
 // Packs [lo, hi), pack lo + i by thread i % nt.
 template <typename T, bool ENT>
 __device__ __noinline__ void grad_plain(const T* row, T* out, int head, int lo, int hi, Coef c, float k, int tid, int nt) {
@@ -536,7 +533,7 @@ __device__ __noinline__ void grad_plain(const T* row, T* out, int head, int lo, 
         uint4 g = fill;
         if (elementwise(c)) {
             const uint4 p = load_pack(src + v);
-            g = c.kind == ROW_SUM ? grad_of<T, ENT>(p, c, k) : grad_of_rare<T, ENT>(p, c, k);
+            g = c.kind == ROW_SUM ? grad_of<T, ENT>(p, c, k) : grad_of_wide<T, ENT>(p, c, k);
         }
         if (same)
             reinterpret_cast<uint4*>(dst)[v] = g;
@@ -572,26 +569,35 @@ __device__ __forceinline__ void remote_store(uint32_t addr, const Part& p) {
 // Sums of one thread's share of a slice against M itself, with differences
 // taken before the multiply: for rows whose maximum is so large, or so low,
 // that l * k - R would keep nothing of t (a row masked throughout). Such rows
-// hold many equal terms, whose roundings share a sign: 64 of them are added in
-// 32 bits, then in 64.
-template <typename T, bool ENT>
+// hold many equal terms, whose roundings share a sign: the sums of each 32 of
+// them are added with the rounding errors carried on.
+// UN: loads in flight; the per-row policy kernel, short of registers, spills
+// more of its short rows' for the sake of 4 (20000 f16 rows of 1000 columns 42.1
+// us against 40.0 with 2; 300 wide fp32 rows of 9001 20.0 and 20.1).
+template <typename T, bool ENT, int UN>
 __device__ __noinline__ Part wide_part(const T* row, int V, float M, float k, int part, int parts, int first, int nt) {
     const Slice sl = slice_of(row, V, part, parts, 0);
     const int v0 = part == 0 ? 0 : sl.head + sl.lo * Type<T>::N, v1 = part == parts - 1 ? V : sl.head + (sl.lo + sl.n) * Type<T>::N;
-    double S = 0.0, Q = 0.0;
+    float s = 0.0f, q = 0.0f, s_off = 0.0f, q_off = 0.0f;
+    const auto carry = [](float& sum, float& off, float x) {
+        const float y = x - off, z = sum + y;
+        off = (z - sum) - y;
+        sum = z;
+    };
     for (int v = v0 + first; v < v1;) {
-        float s = 0.0f, q = 0.0f;
-        const int end = v1 - v > 64 * nt ? v + 64 * nt : v1;
-#pragma unroll 4
+        float ps = 0.0f, pq = 0.0f;
+        const int end = v1 - v > 32 * nt ? v + 32 * nt : v1;
+#pragma unroll UN
         for (; v < end; v += nt) {
             const float t = (widen1(row[v]) - M) * k;
             const float e = ex2_approx(t);
-            s += e;
-            if (ENT) q = fmaf(e, fmaxf(t, -200.0f), q);
+            ps += e;
+            if (ENT) pq = fmaf(e, fmaxf(t, -200.0f), pq);
         }
-        S += (double)s, Q += (double)q;
+        carry(s, s_off, ps);
+        if (ENT) carry(q, q_off, pq);
     }
-    return Part{M, (float)warp_sum(S), ENT ? (float)warp_sum(Q) : 0.0f, 0.0f};
+    return Part{M, warp_sum(s), ENT ? warp_sum(q) : 0.0f, 0.0f};
 }
 
 // Joins such parts.
@@ -723,7 +729,7 @@ __global__ void __launch_bounds__(NT * ROWS, 1024 / (NT * ROWS)) rows_kernel(con
         sync();
         if (!again) break;
         wide = wide_m;
-        mine = wide_part<T, ENT>(row, a.V, wide, k, rank, C, tid, NT);
+        mine = wide_part<T, ENT, POLICY ? 2 : 4>(row, a.V, wide, k, rank, C, tid, NT);
         sync();  // again and wide_m are written once more
     }
     if (rank == 0 && tid == 0) write_row<ENT, POLICY>(a, r, w, in);
@@ -760,7 +766,7 @@ __global__ void __launch_bounds__(NT * ROWS, 1024 / (NT * ROWS)) rows_kernel(con
         grad_plain<T, ENT>(row, out, s.head, s.lo, s.lo + s.n, c, k, tid, NT);
     }
     // the thread that wrote the target's pack puts the target right
-    if (hot >= 0 && hot < s.n && tid == hot_thread && elementwise(c)) put1(out + target, grad_target<ENT>(c, c.lt, k));
+    if (hot >= 0 && hot < s.n && tid == hot_thread && elementwise(c)) put1(out + target, grad1<ENT>(c, c.lt, k) + c.one);
 }
 
 // ---- a stream of rows per cluster ----------------------------------------------
@@ -816,20 +822,18 @@ __device__ __forceinline__ void send_part(uint32_t addr, uint32_t bar, const Par
 }
 
 // Waits for a phase of `bar`. After `limit` cycles, or once another wait of the
-// CTA has given up, returns false: what the CTA has not computed by then comes
-// out NaN. (From then on a phase may be taken for another, so that a later wait
-// says true: rows are looked up by *abort as well.)
-__device__ __forceinline__ bool stream_wait(uint32_t bar, uint32_t parity, volatile int* abort, long long limit) {
-    if (mbar_try_wait(bar, parity)) return true;
+// CTA has given up, returns all the same: the sums that the CTA has not handed
+// in come out NaN, and all its gradients.
+__device__ __forceinline__ void stream_wait(uint32_t bar, uint32_t parity, volatile int* abort, long long limit) {
+    if (mbar_try_wait(bar, parity)) return;
     const long long t0 = clock64();
     while (!mbar_try_wait(bar, parity)) {
-        if (*abort) return false;
+        if (*abort) return;
         if (clock64() - t0 > limit) {
             *abort = 1;
-            return false;
+            return;
         }
     }
-    return true;
 }
 
 // Waits until the part with this tag has landed (0: none was sent).
@@ -990,12 +994,12 @@ __global__ void __launch_bounds__(Shape::NT + 64, Shape::CTAS) stream_kernel(con
                 next_in = inputs(next);
             }
             stream_wait(obar_u + 8 * par, (phases >> par) & 1, abort, a.wait);
+            const bool gone = *abort;  // nothing is sent, and no barrier armed again, once a wait has given up
             Row w = join_parts<ENT>(sh.own[par], NW, k);
             if (C > 1) {
-                // nothing is sent, and no barrier armed again, once a wait has given up
-                if (lane == 0 && !*abort) mbar_arrive_tx(xbar_u + 8 * par, C * 16);
+                if (lane == 0 && !gone) mbar_arrive_tx(xbar_u + 8 * par, C * 16);
                 __syncwarp();
-                if (lane < C && !*abort) {
+                if (lane < C && !gone) {
                     sent = i + 1;
                     send_part(map_rank(smem_u32(&sh.parts[par][rank]), lane), map_rank(xbar_u + 8 * par, lane),
                               Part{w.M, (float)w.S, (float)w.Q, __int_as_float(sent)});
@@ -1007,7 +1011,7 @@ __global__ void __launch_bounds__(Shape::NT + 64, Shape::CTAS) stream_kernel(con
             if (*abort) w.S = NAN, w.wide = false;
             if (w.wide) {  // the same in every CTA: once more through the slices, by these warps
                 const T* row = (const T*)a.logits + r * a.ld;
-                Part own = wide_part<T, ENT>(row, a.V, w.M, k, rank, C, lane, 32);
+                Part own = wide_part<T, ENT, 4>(row, a.V, w.M, k, rank, C, lane, 32);
                 if (lane == 0 && !*abort) mbar_arrive_tx(wbar_u, C * 16);
                 __syncwarp();
                 if (lane < C && !*abort) {
@@ -1067,12 +1071,11 @@ __global__ void __launch_bounds__(Shape::NT + 64, Shape::CTAS) stream_kernel(con
                 stream_wait(cbar_u + 8 * (par ^ 1), (cphase >> (par ^ 1)) & 1, abort, a.wait);
                 cphase ^= 1u << (par ^ 1);
                 c = sh.coef[par ^ 1];
-                if (*abort) c.kind = ROW_NAN;
                 have_c = true;
             };
             for (int j = 0; j < steps; j++) {
                 if (j < n) {
-                    if (!stream_wait(full_u + 8 * stage, phase, abort, a.wait)) c.kind = ROW_NAN;
+                    stream_wait(full_u + 8 * stage, phase, abort, a.wait);
                     const uint32_t at = ring_u + stage * CH + tid * 16;
                     uint4 p[PP];
                     if (j + 1 < n) {
@@ -1103,7 +1106,7 @@ __global__ void __launch_bounds__(Shape::NT + 64, Shape::CTAS) stream_kernel(con
                 if (j >= lag && j - lag < b_n) {
                     want_c();
                     const int base = (j - lag) * CHP + tid;
-                    if (!stream_wait(full_u + 8 * stage, phase, abort, a.wait)) c.kind = ROW_NAN;
+                    stream_wait(full_u + 8 * stage, phase, abort, a.wait);
                     const uint32_t at = ring_u + stage * CH + tid * 16;
                     uint4* d = reinterpret_cast<uint4*>(b_dst) + base;
                     if (same && c.kind == ROW_SUM && j - lag + 1 < b_n) {
@@ -1114,7 +1117,7 @@ __global__ void __launch_bounds__(Shape::NT + 64, Shape::CTAS) stream_kernel(con
                         for (int u = 0; u < PP; u++)
                             if (base + u * NT < b.n) {
                                 const uint4 p = lds_pack(at + u * NT * 16);
-                                const uint4 g = c.kind == ROW_SUM ? grad_of<T, ENT>(p, c, k) : elementwise(c) ? grad_of_rare<T, ENT>(p, c, k) : fill_pack<T>(c);
+                                const uint4 g = c.kind == ROW_SUM ? grad_of<T, ENT>(p, c, k) : c.kind == ROW_WIDE ? grad_of_wide<T, ENT>(p, c, k) : fill_pack<T>(c);
                                 if (same)
                                     __stcs(d + u * NT, g);
                                 else
@@ -1129,29 +1132,32 @@ __global__ void __launch_bounds__(Shape::NT + 64, Shape::CTAS) stream_kernel(con
             if (i > 0) {
                 want_c();
                 if (b.edge >= 0) put_edge<T, ENT>(b_out, b.edge, b_target, b_edge, c, k);
-                // the thread that wrote the target's pack puts the target right (NaN, too: its pack may
-                // be from before a wait gave up)
+                // the thread that wrote the target's pack puts the target right
                 const int hot = b_target >= b.head ? (b_target - b.head) / N - b.lo : -1;
-                if (hot >= 0 && hot < b.n && hot % NT == tid && c.kind != ROW_ZERO)
-                    put1(b_out + b_target, c.kind == ROW_NAN ? NAN : grad_target<ENT>(c, c.lt, k));
+                if (hot >= 0 && hot < b.n && hot % NT == tid && elementwise(c)) put1(b_out + b_target, grad1<ENT>(c, c.lt, k) + c.one);
             }
             if (more) {
                 b_out = (T*)a.grad + r * a.grad_ld;
                 b = s, b_n = n, b_edge = edge, b_target = a.targets[r];
             }
         }
+        const auto fill = [&](int64_t r, int part, int parts, bool nan) {
+            const T* row = (const T*)a.logits + r * a.ld;
+            T* out = (T*)a.grad + r * a.grad_ld;
+            const Slice s = slice_of(row, a.V, part, parts, tid);
+            const Coef c = fill_coef(nan);
+            if (s.edge >= 0) put_edge<T, ENT>(out, s.edge, -1, 0.0f, c, k);
+            grad_plain<T, ENT>(row, out, s.head, s.lo, s.lo + s.n, c, k, tid, NT);
+        };
+        // a thread whose wait gave up has written what the ring held: NaN over all that it has written
+        if (*abort)
+            for (int i = 0; i < mine_n; i++) fill(nth_row(sh, a.rows, cid + i * step, false), rank, C, true);
         // rows that take no part: zeros, or NaN for a target out of range
         for (int j = (int)blockIdx.x; j < a.rows - sh.nlive; j += (int)gridDim.x) {
             const int64_t r = nth_row(sh, a.rows, j, true);
-            const int target = a.targets[r];
-            const bool nan = target >= a.V && !(a.weight && a.weight[r] == 0.0f);
+            const bool nan = a.targets[r] >= a.V && !(a.weight && a.weight[r] == 0.0f);
             if (tid == 0) blank_row<true>(a, r, nan ? NAN : 0.0f);
-            const T* row = (const T*)a.logits + r * a.ld;
-            T* out = (T*)a.grad + r * a.grad_ld;
-            const Slice s = slice_of(row, a.V, 0, 1, tid);
-            const Coef c = fill_coef(nan);
-            if (s.edge >= 0) put_edge<T, ENT>(out, s.edge, target, 0.0f, c, k);
-            grad_plain<T, ENT>(row, out, s.head, 0, s.n, c, k, tid, NT);
+            fill(r, 0, 1, nan);
         }
     }
     // no CTA leaves while a peer may still store into its shared memory, or
@@ -1227,7 +1233,7 @@ __global__ void __launch_bounds__(256, 6) grad_kernel(const Args a, const int pa
     } else {
         grad_plain<T, ENT>(row, out, s.head, s.lo, s.lo + s.n, c, k, tid, NT);
     }
-    if (mine) put1(out + target, grad_target<ENT>(c, lt, k));
+    if (mine) put1(out + target, grad1<ENT>(c, target_logit(c, lt), k) + c.one);
 }
 
 // ---- pairs and sums --------------------------------------------------------------
