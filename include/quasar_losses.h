@@ -22,8 +22,9 @@
  * Rows. Row r of `rows` holds V logits at d_logits + r*ld (elements of dtype,
  * ld >= V, 1 <= V <= QUASAR_MAX_VOCAB, any alignment that the type has).
  * d_targets[r] is its token:
- *   target < 0      the row takes no part: its logits are not read, its
- *                   outputs are 0 and its gradient is a row of zeros;
+ *   target < 0      the row takes no part: its logits do not count (some
+ *                   of them may be read), its outputs are 0 and its
+ *                   gradient is a row of zeros;
  *   target >= V     the row's outputs and its gradient are NaN (the gradient
  *                   zeros in a row of weight 0, in a pair that takes no part
  *                   and outside of the sequences).
@@ -36,14 +37,21 @@
  *   p_v      = exp((l_v - M) / temperature) / S
  *   logprob  = (l_target - M) / temperature - ln S
  *   entropy  = -sum p ln p
- * Sums are kept in 32 bits within a warp and in 64 bits across warps;
- * log-probabilities, entropies and losses are formed in 64 bits from them and
- * rounded once; gradients are formed in 32 bits and rounded once to dtype. A row whose derivatives by
- * log-probability and entropy are both 0 (a clipped ratio) has a gradient of
- * zeros, whatever its logits. A derivative by the log-probability that is
- * infinite or passes 1e38 * temperature gives infinities with their signs where
- * p is not 0, and zeros where it is (one by the entropy: nothing defined where p
- * is not 0). */
+ * Sums over a row are kept in 32 bits by each thread and warp (V / 512 terms a
+ * lane and CTA) and joined in 64 bits, where a row has more than 32 warps of up
+ * to two of them added in 32; the policy loss of many long rows rounds each
+ * CTA's sums to 32 bits before it joins a row's CTAs. From them
+ * log-probabilities, entropies and row losses are formed in 64 bits and rounded
+ * once; sums over sequences and rows are 64-bit sums of these rounded values.
+ * Gradients, and the ratio and KL factor in them, are formed in 32 bits and
+ * rounded once to dtype. So log-probabilities are good to about 4e-7 of 1 +
+ * |logprob| (2^20 equal logits: 2e-5), entropies to 4e-6 of 1 + H (where one
+ * logit holds most of a row: 2e-5).
+ * A row whose derivatives by log-probability and entropy are both 0 (a clipped
+ * ratio) has a gradient of zeros, whatever its logits. Where a derivative by the
+ * log-probability is infinite, or so large that its products pass the fp32
+ * range, the gradient is infinite with its sign where they do, and 0 where p is
+ * 0 (an infinite derivative by the entropy defines nothing where p is not 0). */
 #ifndef QUASAR_LOSSES_H
 #define QUASAR_LOSSES_H
 

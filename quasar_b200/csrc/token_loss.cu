@@ -624,12 +624,13 @@ __device__ __forceinline__ void wait_before() { asm volatile("griddepcontrol.wai
 // (or one CTA) per row, each CTA a slice of it. The sums come from memory; for
 // the gradient the slice is read again, from L2 (or not at all: the last
 // batch of packs is still in registers, which is all of a short slice).
-// Measured at V = 151936: 8191 bf16 rows, a tenth of them left out, in 325 us
-// (1.05 of the measured copy rate: reads are a little faster than copies); one fp32
-// row in 6.2 us.
+// Measured at V = 151936: 8191 bf16 rows, a tenth of them left out, in 313 us
+// (1.09 of the measured copy rate: reads are faster than copies); one fp32
+// row in 4.4 us.
 // With ROWS > 1 (NT = 32) a CTA's warps take a row each: short rows by CTAs of
-// one warp are bound by the rate at which CTAs start, 2.1 ns each (20000 f16
-// rows of 1000 columns: 47.6 us with one row a CTA, 15.9 with 8).
+// their own are bound by the rate at which CTAs start (20000 f16
+// rows of 1000 columns: 53.8 us with a CTA of 128 threads a row, 16.0 with 8 rows
+// a CTA).
 template <typename T, bool ENT, bool POLICY, int NT, int ROWS>
 __global__ void __launch_bounds__(NT * ROWS, 1024 / (NT * ROWS)) rows_kernel(const Args a) {
     static_assert(ROWS == 1 || NT == 32, "a row for each warp, or the CTA's threads for one row");
@@ -781,8 +782,12 @@ __global__ void __launch_bounds__(NT * ROWS, 1024 / (NT * ROWS)) rows_kernel(con
 // sums travel to the joining warp and back while the consumers are busy, and
 // loads of one row stand beside stores of another.
 //
-// The rows in flight have to stay in L2 between their two readings: the
-// launcher takes the cluster size that keeps them under STREAM_L2 bytes.
+// The rows in flight, two per cluster (the one summed and the one before), have
+// to stay in L2 (126 MB) between their two readings. The launcher takes the
+// cluster size that brings one row per cluster under STREAM_L2 bytes, so twice
+// that in flight; with 8 CTAs a row, the most, rows above 1.8 MB pass it (18
+// clusters of 4 MB rows: 75 MB, and twice that), and middle rows, a CTA each, are
+// 296 of up to 128 KB (39 MB, and twice that).
 // Rows that take no part are left out of the stream (a bit per row in shared
 // memory), so that every cluster gets the same number of live rows, and are
 // filled at the end.
@@ -1178,11 +1183,11 @@ __global__ void __launch_bounds__(Shape::NT + 64, Shape::CTAS) stream_kernel(con
 // ---- the gradient from given sums -------------------------------------------------
 
 // One CTA per slice of a row, `parts` of them in turn: one read and one write.
-// Measured: 2047 bf16 rows of 151936, a fifth of them zeros, in 177 us (0.97
+// Measured: 2047 bf16 rows of 151936, a fifth of them zeros, in 178 us (0.96
 // of the measured copy rate) with slices of 76 KB; slices of a quarter of
-// that, in which a CTA's start weighs more, take 234 us.
+// that, in which a CTA's start weighs more, take 182 us.
 // ROWS > 1: a warp for each row, for short ones (20000 f16 rows of 1000
-// columns: 56 us with a CTA for each, 20 with a warp).
+// columns: 60 us with a CTA for each, 20 with a warp).
 template <typename T, bool ENT, int ROWS>
 __global__ void __launch_bounds__(256, 6) grad_kernel(const Args a, const int parts) {
     constexpr int N = Type<T>::N, NT = 256 / ROWS;
@@ -1374,8 +1379,8 @@ static cudaError_t launch(void (*kern)(P...), unsigned grid, int block, size_t s
 static constexpr int SMS = 148;
 
 // CTAs per row: clusters of up to 8 while the rows alone leave SMs idle, and
-// the slices are not under 8 KB. At V = 151936, fp32: 1 row 6.2 us with 8
-// CTAs and 22 with one; 256 rows 28.7 us with 2, 31.1 with 1, 33.7 with 4.
+// the slices are not under 8 KB. At V = 151936, fp32: 1 row 4.4 us with 8
+// CTAs and 10.8 with one; 256 rows 26.7 us with 2, 30.6 with 1, 29.8 with 4.
 static int row_cluster(int64_t rows, int64_t row_bytes) {
     int C = 1;
     while (C < MAXC && rows * C < 2 * SMS && row_bytes >= (int64_t)C * 2 * 8192) C *= 2;
@@ -1389,14 +1394,14 @@ static cudaError_t rows_launch(const Args& a, int C, cudaStream_t st) {
 }
 
 // Rows that a warp takes alone, in bytes: 20000 bf16 rows of 4000 columns,
-// policy loss and gradient, 80 us against 110 with 128 threads a row; 500 rows
-// of 18 KB 13.1 against 9.4.
+// policy loss and gradient, 78 us against 112 with 128 threads a row; 500 rows
+// of 18 KB 17.4 against 11.4.
 static constexpr int64_t ROW_SHORT = 8192;
 
 // Short rows take small CTAs, of which an SM runs more at once: a CTA's start,
 // its barrier and its scalars take about 4 us whatever its slice. bf16 rows of
-// 38 KB, 16384 of them: 247 us with 128 threads, 274 with 256 (policy loss and
-// gradient); fp32 rows of 76 KB, 2000 of them: 63 us with 256, 70 with 128.
+// 38 KB, 16384 of them: 255 us with 128 threads, 274 with 256 (policy loss and
+// gradient); fp32 rows of 76 KB, 2000 of them: 62 us with 256, 69 with 128.
 template <typename T, bool ENT, bool POLICY>
 static cudaError_t rows_by_size(const Args& a, cudaStream_t st) {
     const int64_t row_bytes = (int64_t)a.V * sizeof(T);
@@ -1408,10 +1413,11 @@ static cudaError_t rows_by_size(const Args& a, cudaStream_t st) {
 
 // Long rows: one CTA of 640 consumers per SM with chunks of 30 KB, and of 448
 // with chunks of 28 KB for the entropy of 16-bit types, which is bound by
-// instructions and gains from 119 registers a thread instead of 80 (bf16,
-// V = 151936, 2000 rows 256 us against 276, 1023 rows 116 and 123; V = 200000,
-// 1500 rows 236 and 265). Without entropy 640 are faster (V = 200000, 220 and
-// 227), and in fp32, bound by memory (2000 rows with entropy 399 and 418).
+// instructions and has 119 registers a thread instead of 80 (bf16, long runs:
+// V = 200000, 1500 rows 251 us against 261; V = 100000, 3000 rows 253 and 258;
+// about even at V = 151936, 2000 rows 268 and 264, 1023 rows with KL term 116 and
+// 113). Without entropy the two are even (V = 200000, 216), and in fp32, bound by
+// memory, 640 are faster (2000 rows with entropy 391 and 405).
 // Middle rows, of which an SM can hold two: two CTAs of 256 with chunks of 20 KB.
 template <typename T, bool ENT>
 using StreamLong =
@@ -1472,9 +1478,10 @@ static cudaError_t stream_launch(const Args& a, int C, cudaStream_t st) {
 
 // The policy loss with its gradient: the streaming kernel where a row is long
 // enough for its chunks and there are rows for several turns of every cluster
-// (policy loss and gradient at V = 151936: fp32, 4096 rows 803 us streamed,
-// 899 with a cluster of 8 per row; bf16, 600 rows 82 and 88 us, 148 rows 27
-// and 29; 50021 f16 columns, 1000 rows 47 and 52 us, 300 rows 25 and 22).
+// (policy loss and gradient at V = 151936: fp32, 4096 rows 745 us streamed,
+// 1040 with a CTA per row; bf16, 600 rows 79 to 87 and 102 us, 148 rows 28 to 29
+// and 27; 50021 f16 columns, 3001 rows 118 and 131 us, 1000 rows 48 and 51, 300
+// rows 25.7 and 21.8).
 template <typename T, bool ENT>
 static cudaError_t policy_by_size(const Args& a, cudaStream_t st) {
     const int64_t row_bytes = (int64_t)a.V * sizeof(T);

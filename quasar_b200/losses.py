@@ -162,7 +162,7 @@ def token_logprobs(logits, targets, *, temperature: float = 1.0, entropy: bool =
                    out: Optional[TokenLogprobs] = None, stream=None) -> TokenLogprobs:
     """Log-probability of each row's target under softmax(logits / temperature), and on request the row's entropy.
 
-    targets: [rows] int32; below 0: the row is not read and its outputs are 0.
+    targets: [rows] int32; below 0: the row takes no part and its outputs are 0.
     out: a TokenLogprobs of an earlier call whose tensors are written again (its entropy as ``entropy`` asks).
     Launches on ``stream`` (a torch.cuda.Stream; default: the current stream).
     """
