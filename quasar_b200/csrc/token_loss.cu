@@ -400,7 +400,7 @@ __device__ __forceinline__ Coef row_coef(const Args& a, const Row& w, const RowI
     float loss, g = policy_slope<float>(lo, hi, kl, in.adv, ratio, eu, &loss) * ws;
     if (!finite(g) && d == d && u == u) {
         const bool out = in.adv == 0.0f || (in.adv > 0.0f ? ratio > hi : ratio < lo);
-        g = (out ? 0.0f : -steep((float)d, in.adv, ws)) - (steep((float)u, kl, ws) - kl * ws);
+        g = ws == 0.0f ? 0.0f : (out ? 0.0f : -steep((float)d, in.adv, ws)) - (steep((float)u, kl, ws) - kl * ws);
     }
     Coef c = make_coef(w.M, (float)w.R, w.wide, S, ENT ? (float)-LN2 * ((float)w.Q / S) : 0.0f, g, ENT ? -(float)a.ec * ws : 0.0f, (float)a.inv_t);
     c.lt = target_logit(c, in.lt);

@@ -330,3 +330,15 @@ def test_entropies(case):
     assert (err.abs() <= bound).all(), f"off by {err.abs().max().item():.3g}, {(err.abs() / bound).max().item():.3g} of the bound"
     assert (err.abs().median() <= bound.median() / 4).all(), f"median {err.abs().median().item():.3g}"
     assert err.mean().abs().item() <= 2e-7 + 4 * err.std().item() / math.sqrt(rows), f"mean {err.mean().item():.3g}"
+
+
+@pytest.mark.parametrize("shape", [(40, 1000), (600, 30001)], ids=str)
+def test_scale_of_zero(shape):
+    """A gradient scaled by 0 is zeros, of ratios and KL factors beyond fp32, too."""
+    rows, V = shape
+    logits, targets, g = rows_of(rows, V, torch.float32, 87)
+    lp, _ = reference(logits, targets, 1.0)
+    one = torch.ones(rows, device="cuda")
+    for far in (1.0, 110.0, 800.0):
+        out = q().policy_loss(logits, targets, (lp - far).float(), -one, ref_logprob=(lp + far).float(), kl_coef=0.1, grad_scale=0.0)
+        assert (out.grad == 0).all()
