@@ -135,11 +135,11 @@ int quasar_policy_loss(const void* d_logits, int dtype, int64_t ld, int rows, in
                        d_weight, params, d_logprob, d_entropy, d_row_loss, d_loss, d_grad, grad_ld, stream);
 }
 
-int quasar_selftest_stalled_policy_loss(int64_t wait_cycles, int chunks, const void* d_logits, int dtype, int64_t ld, int rows, int V,
-                       const int32_t* d_targets,
-                       const float* d_old_logprob, const float* d_advantage, const float* d_ref_logprob,
-                       const float* d_weight, const quasar_policy_params* params, float* d_logprob, float* d_entropy,
-                       float* d_row_loss, float* d_loss, void* d_grad, int64_t grad_ld, void* stream) {
+int quasar_selftest_stalled_policy_loss(int64_t wait_cycles, int chunks, const void* d_logits, int dtype, int64_t ld,
+                                        int rows, int V, const int32_t* d_targets, const float* d_old_logprob,
+                                        const float* d_advantage, const float* d_ref_logprob, const float* d_weight,
+                                        const quasar_policy_params* params, float* d_logprob, float* d_entropy,
+                                        float* d_row_loss, float* d_loss, void* d_grad, int64_t grad_ld, void* stream) {
     if (wait_cycles < 0 || wait_cycles > qs::WAIT_CYCLES || chunks < 0) return QUASAR_EINVAL;
     return policy_loss(wait_cycles, chunks, d_logits, dtype, ld, rows, V, d_targets, d_old_logprob, d_advantage, d_ref_logprob,
                        d_weight, params, d_logprob, d_entropy, d_row_loss, d_loss, d_grad, grad_ld, stream);

@@ -282,9 +282,9 @@ WIDE_ROWS = [(160, torch.float32), (300, torch.float32)]
 @pytest.mark.parametrize("rows,dtype", WIDE_ROWS)
 def test_sums_of_wide_rows(rows, dtype):
     """Rows masked throughout by a value near -1.5e7, where logits stand a whole number apart, at the largest vocabulary:
-    millions of equal terms, whose roundings all have one sign. At most 64 of them are added in 32 bits (a lane's
-    partial sum), then in 64: 64 * 2^-24 for the additions, (4 + 3 |t|) 2^-24 for a term with |t| < 2, and 4 roundings
-    of parts and of the logarithm."""
+    millions of equal terms, whose roundings all have one sign. At most 64 roundings add up (32 terms of a lane, whose
+    sums are added with the errors carried on, then 32 lanes): 64 * 2^-24 for the additions, (4 + 3 |t|) 2^-24 for a
+    term with |t| < 2, and 4 roundings of parts and of the logarithm."""
     V = 1 << 20
     logits = torch.full((rows, V), -1.5e7 - 1, dtype=dtype, device="cuda")
     logits[:, 12345] = -1.5e7

@@ -141,3 +141,12 @@ def test_parameter_records_match_the_header():
     from quasar_b200.losses import PolicyParams, PreferenceParams
     assert ctypes.sizeof(PolicyParams) == 24
     assert ctypes.sizeof(PreferenceParams) == 24
+
+
+@pytest.mark.parametrize("wait,chunks", [(-1, 0), ((1 << 32) + 1, 0), (1, -1)])
+def test_self_test_arguments_are_checked(wait, chunks):
+    from quasar_b200.losses import PolicyParams
+    rec = PolicyParams(1.0, 0.2, 0.2, 0.0, 0.0, 1.0)
+    assert _lib().quasar_selftest_stalled_policy_loss(wait, chunks, P(4096), 0, 16, 2, 16, P(64), P(64), P(64), None, None,
+                                                      ctypes.addressof(rec), P(64), None, P(64), P(64), P(8192), 16,
+                                                      None) == EINVAL
