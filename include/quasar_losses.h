@@ -185,10 +185,10 @@ int quasar_preference_loss(const void *d_logits, int dtype, int64_t ld, int rows
 
 /* ---- self-test ------------------------------------------------------------ */
 
-/* quasar_policy_loss with waits of at most wait_cycles (0 to 2^32), of which
- * one CTA's loads stop after `chunks` chunks where the call takes the streaming
- * kernel (many long rows, with d_grad): waits run out there. Used by the GPU
- * tests to see that what was not computed comes out NaN. */
+/* quasar_policy_loss with waits of about wait_cycles (0 to 2^32, rounded down to
+ * a power of two), of which one CTA's loads stop after `chunks` chunks where the
+ * call takes the streaming kernel (many long rows, with d_grad): waits run out
+ * there. Used by the GPU tests to see that what was not computed comes out NaN. */
 int quasar_selftest_stalled_policy_loss(int64_t wait_cycles, int chunks,
                                         const void *d_logits, int dtype, int64_t ld, int rows, int V,
                                         const int32_t *d_targets, const float *d_old_logprob, const float *d_advantage,

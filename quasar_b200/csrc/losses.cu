@@ -42,8 +42,6 @@ qs::loss::Args row_args(const void* d_logits, int64_t ld, int rows, int V, const
     a.targets = d_targets;
     a.inv_t = 1.0 / (double)temperature;
     a.k = (float)(1.4426950408889634074 * a.inv_t);
-    a.wait = qs::WAIT_CYCLES;
-    a.stall = -1;
     return a;
 }
 
@@ -54,7 +52,7 @@ int status(cudaError_t e) {
     return QUASAR_ECUDA;
 }
 
-int policy_loss(int64_t wait, int stall, const void* d_logits, int dtype, int64_t ld, int rows, int V, const int32_t* d_targets,
+int policy_loss(uint32_t selftest, const void* d_logits, int dtype, int64_t ld, int rows, int V, const int32_t* d_targets,
                 const float* d_old_logprob, const float* d_advantage, const float* d_ref_logprob,
                 const float* d_weight, const quasar_policy_params* params, float* d_logprob, float* d_entropy,
                 float* d_row_loss, float* d_loss, void* d_grad, int64_t grad_ld, void* stream) {
@@ -84,8 +82,7 @@ int policy_loss(int64_t wait, int stall, const void* d_logits, int dtype, int64_
         a.scale = params->grad_scale;
         a.grad = d_grad;
         a.grad_ld = grad_ld;
-        a.wait = wait;
-        a.stall = stall;
+        a.selftest = selftest;
         const int rc = status(qs::loss::launch_rows(a, dtype, st));
         if (rc != QUASAR_OK) return rc;
     }
@@ -131,7 +128,7 @@ int quasar_policy_loss(const void* d_logits, int dtype, int64_t ld, int rows, in
                        const float* d_old_logprob, const float* d_advantage, const float* d_ref_logprob,
                        const float* d_weight, const quasar_policy_params* params, float* d_logprob, float* d_entropy,
                        float* d_row_loss, float* d_loss, void* d_grad, int64_t grad_ld, void* stream) {
-    return policy_loss(qs::WAIT_CYCLES, -1, d_logits, dtype, ld, rows, V, d_targets, d_old_logprob, d_advantage, d_ref_logprob,
+    return policy_loss(0, d_logits, dtype, ld, rows, V, d_targets, d_old_logprob, d_advantage, d_ref_logprob,
                        d_weight, params, d_logprob, d_entropy, d_row_loss, d_loss, d_grad, grad_ld, stream);
 }
 
@@ -141,7 +138,10 @@ int quasar_selftest_stalled_policy_loss(int64_t wait_cycles, int chunks, const v
                                         const quasar_policy_params* params, float* d_logprob, float* d_entropy,
                                         float* d_row_loss, float* d_loss, void* d_grad, int64_t grad_ld, void* stream) {
     if (wait_cycles < 0 || wait_cycles > qs::WAIT_CYCLES || chunks < 0) return QUASAR_EINVAL;
-    return policy_loss(wait_cycles, chunks, d_logits, dtype, ld, rows, V, d_targets, d_old_logprob, d_advantage, d_ref_logprob,
+    uint32_t bits = 0;
+    while ((2ll << bits) <= wait_cycles) bits++;
+    const uint32_t most = 0xFFFFFEu, stop = (uint32_t)chunks < most ? (uint32_t)chunks : most;
+    return policy_loss(bits << 24 | (stop + 1), d_logits, dtype, ld, rows, V, d_targets, d_old_logprob, d_advantage, d_ref_logprob,
                        d_weight, params, d_logprob, d_entropy, d_row_loss, d_loss, d_grad, grad_ld, stream);
 }
 
@@ -190,7 +190,6 @@ int quasar_preference_loss(const void* d_logits, int dtype, int64_t ld, int rows
     if (rc == QUASAR_OK && rows > 0 && d_grad) {
         a.stats_in = d_stats;
         a.g_lp = d_row_grad;
-        a.zero_is_out = true;
         a.grad = d_grad;
         a.grad_ld = grad_ld;
         rc = status(qs::loss::launch_grad(a, dtype, st));

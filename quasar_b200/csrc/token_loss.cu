@@ -826,12 +826,12 @@ __device__ __forceinline__ void send_part(uint32_t addr, uint32_t bar, const Par
         : "memory");
 }
 
-// Waits for a phase of `bar`. After `limit` cycles, or once another wait of the
+// Waits for a phase of `bar`. After WAIT_CYCLES (or the self-test's limit), or once another wait of the
 // CTA has given up, returns all the same: the sums that the CTA has not handed
 // in come out NaN, and all its gradients.
-__device__ __forceinline__ void stream_wait(uint32_t bar, uint32_t parity, volatile int* abort, long long limit) {
+__device__ __forceinline__ void stream_wait(uint32_t bar, uint32_t parity, volatile int* abort, uint32_t selftest) {
     if (mbar_try_wait(bar, parity)) return;
-    const long long t0 = clock64();
+    const long long t0 = clock64(), limit = selftest ? 1ll << (selftest >> 24) : WAIT_CYCLES;
     while (!mbar_try_wait(bar, parity)) {
         if (*abort) return;
         if (clock64() - t0 > limit) {
@@ -935,13 +935,13 @@ __global__ void __launch_bounds__(Shape::NT + 64, Shape::CTAS) stream_kernel(con
             asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(again));
             asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(once));
             uint32_t stage = 0, phase = 0, issued = 0;
-            const uint32_t stop = cid == 0 && rank == C - 1 ? (uint32_t)a.stall : ~0u;
+            const uint32_t stop = a.selftest && cid == 0 && rank == C - 1 ? (a.selftest & 0xFFFFFFu) - 1 : ~0u;
             const uint4* b_src = nullptr;  // the row before, whose gradient is due
             int b_n = 0, b_packs = 0;
             const auto put = [&](const uint4* src, int j, int packs, uint64_t pol) {
                 const uint32_t bytes = (uint32_t)min(CHP, packs - j * CHP) * 16;
                 if (issued == stop) return;
-                stream_wait(empty_u + 8 * stage, phase ^ 1, abort, a.wait);
+                stream_wait(empty_u + 8 * stage, phase ^ 1, abort, a.selftest);
                 if (*abort) return;
                 mbar_arrive_tx(full_u + 8 * stage, bytes);
                 bulk_load(ring_u + stage * CH, src + j * CHP, bytes, full_u + 8 * stage, pol);
@@ -998,7 +998,7 @@ __global__ void __launch_bounds__(Shape::NT + 64, Shape::CTAS) stream_kernel(con
                 next = nth_row(sh, a.rows, cid + (i + 1) * step, false);
                 next_in = inputs(next);
             }
-            stream_wait(obar_u + 8 * par, (phases >> par) & 1, abort, a.wait);
+            stream_wait(obar_u + 8 * par, (phases >> par) & 1, abort, a.selftest);
             const bool gone = *abort;  // nothing is sent, and no barrier armed again, once a wait has given up
             Row w = join_parts<ENT>(sh.own[par], NW, k);
             if (C > 1) {
@@ -1009,7 +1009,7 @@ __global__ void __launch_bounds__(Shape::NT + 64, Shape::CTAS) stream_kernel(con
                     send_part(map_rank(smem_u32(&sh.parts[par][rank]), lane), map_rank(xbar_u + 8 * par, lane),
                               Part{w.M, (float)w.S, (float)w.Q, __int_as_float(sent)});
                 }
-                stream_wait(xbar_u + 8 * par, (phases >> par) & 1, abort, a.wait);
+                stream_wait(xbar_u + 8 * par, (phases >> par) & 1, abort, a.selftest);
                 w = join_parts<ENT>(sh.parts[par], C, k);
             }
             phases ^= 1u << par;
@@ -1023,7 +1023,7 @@ __global__ void __launch_bounds__(Shape::NT + 64, Shape::CTAS) stream_kernel(con
                     own.tag = __int_as_float(++wide_sent);
                     send_part(map_rank(smem_u32(&sh.wide_parts[rank]), lane), map_rank(wbar_u, lane), own);
                 }
-                stream_wait(wbar_u, wphase, abort, a.wait);
+                stream_wait(wbar_u, wphase, abort, a.selftest);
                 wphase ^= 1;
                 w = join_wide(sh.wide_parts, C, w.M, k);
                 if (*abort) w.S = NAN;
@@ -1058,7 +1058,7 @@ __global__ void __launch_bounds__(Shape::NT + 64, Shape::CTAS) stream_kernel(con
             float edge = -INFINITY;
             int n = 0;
             if (more) {  // the row's number comes with its first chunk
-                stream_wait(full_u + 8 * stage, phase, abort, a.wait);
+                stream_wait(full_u + 8 * stage, phase, abort, a.selftest);
                 r = *abort ? nth_row(sh, a.rows, cid + i * step, false) : *(volatile int*)&sh.rows[i & 7];
                 row = (const T*)a.logits + r * a.ld;
                 s = slice_of(row, a.V, rank, C, tid);
@@ -1073,14 +1073,14 @@ __global__ void __launch_bounds__(Shape::NT + 64, Shape::CTAS) stream_kernel(con
             const bool same = ((uintptr_t)b_dst & 15) == 0;
             const auto want_c = [&]() {  // the coefficients of the row before
                 if (have_c) return;
-                stream_wait(cbar_u + 8 * (par ^ 1), (cphase >> (par ^ 1)) & 1, abort, a.wait);
+                stream_wait(cbar_u + 8 * (par ^ 1), (cphase >> (par ^ 1)) & 1, abort, a.selftest);
                 cphase ^= 1u << (par ^ 1);
                 c = sh.coef[par ^ 1];
                 have_c = true;
             };
             for (int j = 0; j < steps; j++) {
                 if (j < n) {
-                    stream_wait(full_u + 8 * stage, phase, abort, a.wait);
+                    stream_wait(full_u + 8 * stage, phase, abort, a.selftest);
                     const uint32_t at = ring_u + stage * CH + tid * 16;
                     uint4 p[PP];
                     if (j + 1 < n) {
@@ -1111,7 +1111,7 @@ __global__ void __launch_bounds__(Shape::NT + 64, Shape::CTAS) stream_kernel(con
                 if (j >= lag && j - lag < b_n) {
                     want_c();
                     const int base = (j - lag) * CHP + tid;
-                    stream_wait(full_u + 8 * stage, phase, abort, a.wait);
+                    stream_wait(full_u + 8 * stage, phase, abort, a.selftest);
                     const uint32_t at = ring_u + stage * CH + tid * 16;
                     uint4* d = reinterpret_cast<uint4*>(b_dst) + base;
                     if (same && c.kind == ROW_SUM && j - lag + 1 < b_n) {
@@ -1203,7 +1203,7 @@ __global__ void __launch_bounds__(256, 6) grad_kernel(const Args a, const int pa
     const T* row = (const T*)a.logits + r * a.ld;
     T* out = (T*)a.grad + r * a.grad_ld;
     const Slice s = slice_of(row, a.V, part, ROWS == 1 ? parts : 1, tid);
-    Coef c = fill_coef(target >= a.V && !(a.zero_is_out && g_lp == 0.0f));
+    Coef c = fill_coef(target >= a.V && !(a.row_grad && g_lp == 0.0f));
     if (target >= 0 && target < a.V) {
         const float R = rintf(st.max * k);
         const bool wide = !(fabsf(R) < WIDE) && !isinf(st.max);

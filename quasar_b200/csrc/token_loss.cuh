@@ -16,6 +16,10 @@ struct Args {
     int rows, V;
     const int32_t* targets;
     float k;       // log2(e) / temperature: exp((l - M) / T) = 2^((l - M) * k)
+    // streaming kernel's self-test, else 0: its waits end after 2^(high 8 bits)
+    // cycles, and one CTA's loads stop after (low 24 bits) - 1 chunks. (In what
+    // was padding: beyond 216 bytes of arguments a launch takes 0.4 us longer.)
+    uint32_t selftest;
     double inv_t;  // 1 / temperature
 
     float* logprob;
@@ -32,7 +36,9 @@ struct Args {
     float* row_loss;
     double scale;  // gradient scale
 
-    // preference loss: zeroed by the statistics kernel, filled by the pair kernel
+    // preference loss: zeroed by the statistics kernel, filled by the pair kernel;
+    // to the gradient kernel a sign that rows of g_lp 0 take no part, whatever
+    // their target
     float* row_grad;
 
     // gradient (policy: NULL for none)
@@ -42,13 +48,8 @@ struct Args {
     const float* g_ent;      // ... or NULL
     const float* ent_in;     // entropies the statistics kernel gave (with g_ent)
     const quasar_logprob_stat* stats_in;
-    bool zero_is_out;        // g_lp of 0: the row takes no part, whatever its target (preference loss)
-
-    // streaming kernel: the limit of a wait in cycles, and for the self-test
-    // the chunks after which one CTA's loads stop (-1: they do not)
-    long long wait;
-    int stall;
 };
+static_assert(sizeof(Args) == 216, "see selftest");
 
 struct PairArgs {
     const float* logprob;
